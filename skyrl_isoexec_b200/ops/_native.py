@@ -21,7 +21,7 @@ class NativeError(RuntimeError):
     pass
 
 
-_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+_P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_double
 
 _SIGS = {
     "ix_init": [],
@@ -50,6 +50,8 @@ _SIGS = {
     "ix_reduce_sum": [_P, _L, _I, _I, _P, _P, _I, _P],
     "ix_clip_coef": [_P, _F, _P, _P, _P],
     "ix_adamw": [_P, _P, _P, _P, _P, _L, _I, _F, _F, _F, _F, _F, _I, _P, _P],
+    "ix_tensor_adamw_chunk": [],
+    "ix_tensor_adamw": [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _D, _D, _D, _D, _L, _P],
     "ix_accum_bf16_to_f32": [_P, _P, _L, _I, _P],
     "ix_router_topk": [_P, _L, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P],
     "ix_moe_combine": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
