@@ -1,0 +1,624 @@
+// Low-rank adapters of many requests beside a shared projection, with their gradients.
+//
+//   forward     h[t] = s_a (x[t] A_a^T),   out[t] = y[t] + h[t] B_a^T        a = adapter of token t
+//   backward    g[t] = s_a (dy[t] B_a),    dx[t] = g[t] A_a (+ base),        dA_a = sum_t g[t]^T x[t],   dB_a = sum_t dy[t]^T h[t]
+//
+// x [T, K], y / dy [T, N], A [E, r, K], B [E, N, r] bf16, s [E] fp32; r is a multiple of 8 up to 128. Tokens without an
+// adapter keep y (dx: base or zero).
+//
+// The rank is small, so every one of these products is bound by reading and writing the token rows. The forward is one
+// kernel: a cluster of CTAs owns a tile of 16 or 64 tokens of ONE adapter, its warps split K, the partial h are summed in
+// a fixed order through shared and distributed shared memory, and the same warps split N to add h B^T to y. x is read
+// once, y read and out written once, h never goes through memory on the way. The backward's g and dx are the same kernel
+// with the factors read across their rows. h and g are kept in 32 bits until they become operands of the second product:
+// there each is the sum of two bf16 numbers (its rounding and the rest, 16 bits together), so the only rounding to 8 bits
+// that shows is that of the output. Products run on mma.sync, operands straight from global memory in fragments of 16
+// bytes a lane: a contraction may take its elements in any order as long as both operands agree, so a lane's 8 neighbours
+// feed two products of depth 16.
+#include "bw_common.cuh"
+#include "host_util.h"
+
+#include <cooperative_groups.h>
+
+namespace {
+using namespace bw;
+namespace cg = cooperative_groups;
+
+constexpr int kMaxAdapters = 1024;
+constexpr int kMaxRank = 128;
+constexpr int kSmall = 16, kLarge = 64;      // tokens a tile
+
+// ------------------------------------------------------------------------------------------------ plan
+// Stable counting sort of the tokens by adapter (out of range: behind all others) and the tiles of both sizes.
+// One CTA; warp w owns tokens [w per, (w+1) per), so a token's place depends on the ids alone.
+__global__ void __launch_bounds__(1024)
+lora_plan_kernel(const int* __restrict__ ids, int T, int E, int* __restrict__ perm, int* __restrict__ offsets, int4* __restrict__ tiles_s,
+                 int4* __restrict__ tiles_l, int* __restrict__ n_tiles) {
+  extern __shared__ int sm[];                // [warps][E + 1] counts, then first places
+  const int G = E + 1, W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* total = sm + W * G;                   // [G]
+  for (int i = threadIdx.x; i < W * G; i += blockDim.x) sm[i] = 0;
+  __syncthreads();
+  const int per = ((T + W - 1) / W + 31) & ~31;
+  const int lo = min(T, warp * per), hi = min(T, lo + per);
+  int* mine = sm + warp * G;
+  for (int i = lo; i < hi; i += 32) {
+    const bool in = i + lane < hi;
+    int a = in ? ids[i + lane] : -2;
+    if (in && (a < 0 || a >= E)) a = E;
+    const unsigned same = __match_any_sync(0xffffffffu, a);
+    if (in && (same & ((1u << lane) - 1)) == 0) mine[a] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int a = threadIdx.x; a < G; a += blockDim.x) {
+    int run = 0;
+    for (int w = 0; w < W; ++w) {
+      const int c = sm[w * G + a];
+      sm[w * G + a] = run;
+      run += c;
+    }
+    total[a] = run;
+  }
+  __syncthreads();
+  __shared__ int s_off[kMaxAdapters + 2], s_ts[kMaxAdapters + 2], s_tl[kMaxAdapters + 2];
+  if (warp == 0) {                           // first token and first tiles of every group
+    int c0 = 0, c1 = 0, c2 = 0;
+    for (int a0 = 0; a0 < G; a0 += 32) {
+      const int a = a0 + lane;
+      const int n = a < G ? total[a] : 0;
+      int v0 = n, v1 = (n + kSmall - 1) / kSmall, v2 = (n + kLarge - 1) / kLarge;
+      const int u0 = v0, u1 = v1, u2 = v2;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int w0 = __shfl_up_sync(0xffffffffu, v0, d), w1 = __shfl_up_sync(0xffffffffu, v1, d), w2 = __shfl_up_sync(0xffffffffu, v2, d);
+        if (lane >= d) v0 += w0, v1 += w1, v2 += w2;
+      }
+      if (a < G) s_off[a] = c0 + v0 - u0, s_ts[a] = c1 + v1 - u1, s_tl[a] = c2 + v2 - u2;
+      c0 += __shfl_sync(0xffffffffu, v0, 31), c1 += __shfl_sync(0xffffffffu, v1, 31), c2 += __shfl_sync(0xffffffffu, v2, 31);
+    }
+    if (lane == 0) s_off[G] = c0, n_tiles[0] = c1, n_tiles[1] = c2;
+  }
+  __syncthreads();
+  for (int a = threadIdx.x; a <= G; a += blockDim.x) offsets[a] = s_off[a];
+  for (int i = lo; i < hi; i += 32) {
+    const bool in = i + lane < hi;
+    int a = in ? ids[i + lane] : -2;
+    if (in && (a < 0 || a >= E)) a = E;
+    const unsigned same = __match_any_sync(0xffffffffu, a);
+    const int before = __popc(same & ((1u << lane) - 1));
+    int at = 0;
+    if (in) at = mine[a];
+    __syncwarp();
+    if (in && before == 0) mine[a] = at + __popc(same);
+    __syncwarp();
+    if (in) perm[s_off[a] + at + before] = i + lane;
+  }
+  // tiles: (adapter or -1, first place in perm, tokens)
+  for (int a = warp; a < G; a += W) {
+    const int n = total[a], o = s_off[a], id = a < E ? a : -1;
+    for (int i = lane; i * kSmall < n; i += 32) tiles_s[s_ts[a] + i] = make_int4(id, o + i * kSmall, min(kSmall, n - i * kSmall), 0);
+    for (int i = lane; i * kLarge < n; i += 32) tiles_l[s_tl[a] + i] = make_int4(id, o + i * kLarge, min(kLarge, n - i * kLarge), 0);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ fragments
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld16(const __nv_bfloat16* p, bool ok) {
+  return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+}
+// x = hi + lo, two bf16 numbers; packed pairs
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+struct ApplyArgs {
+  const __nv_bfloat16* in;        // [T, K] rows that are contracted (x, or dy)
+  const __nv_bfloat16* base;      // [T, N] added to (y, or the other part of dx); null: nothing
+  __nv_bfloat16* out;             // [T, N]; null: only h is wanted
+  const __nv_bfloat16* down;      // factor of the first product: [E, r, K], or across: [E, K, r]
+  const __nv_bfloat16* up;        // factor of the second: [E, N, r], or across: [E, r, N]
+  const float* scale;             // [E]
+  const int* perm;
+  const int4* tiles;
+  const int* n_tiles;
+  __nv_bfloat16* h;               // [2, T, r] in the plan's order: s h as a bf16 and the rest; may be null
+  long long ld_in, ld_base, ld_out;
+  int T, K, N, r;
+};
+
+constexpr int kWarps = 8;
+// shared memory: partial sums [kWarps / MT][16 MT][8 RT + 4] fp32, their sum [16 MT][8 RT + 4], a warp's 2 KB for factors
+// that are read across
+template <int RT, int MT>
+constexpr int apply_smem(bool across) {
+  return (kWarps / MT + 1) * 16 * MT * (8 * RT + 4) * 4 + (across ? kWarps * 2048 : 0);
+}
+
+// One tile of tokens. MT: 16-row groups of the tile; RT: rank in groups of 8 (r <= 8 RT); ACROSS: factors stored with the
+// contracted index outermost for the first product and innermost for the second (the backward).
+template <int RT, int MT, bool ACROSS>
+__global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_constant__ ApplyArgs p) {
+  constexpr int kSplits = kWarps / MT;                 // warps that share a 16-row group
+  constexpr int LD = 8 * RT + 4;                       // floats a row of h
+  constexpr int KS = RT < 2 ? 1 : RT / 2;              // depth-16 steps over the rank
+  extern __shared__ __align__(16) float smem[];
+  if (blockIdx.y >= p.n_tiles[0]) return;              // the same for the whole cluster
+  const int4 tile = p.tiles[blockIdx.y];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int c = gridDim.x, rank_cta = blockIdx.x;
+  const int mt = warp % MT, ks = warp / MT;
+  const int parts = kSplits * c, part = rank_cta * kSplits + ks;
+  const int r0 = mt * 16 + g, r1 = r0 + 8;             // rows of the tile held by this lane
+  const bool ok0 = r0 < tile.z, ok1 = r1 < tile.z;
+  const long long row0 = p.perm[tile.y + (ok0 ? r0 : 0)], row1 = p.perm[tile.y + (ok1 ? r1 : 0)];
+  const int chunks = (p.N + 31) >> 5;
+  const int n_lo = static_cast<int>(static_cast<long long>(chunks) * part / parts), n_hi = static_cast<int>(static_cast<long long>(chunks) * (part + 1) / parts);
+
+  if (tile.x < 0) {                                    // no adapter: the base alone
+    if (p.out == nullptr || p.out == p.base) return;
+    for (int n = n_lo; n < n_hi; ++n) {
+      const int col = n * 32 + 8 * t;
+      if (col >= p.N) break;
+      if (ok0) *reinterpret_cast<uint4*>(p.out + row0 * p.ld_out + col) = ld16(p.base + row0 * p.ld_base + col, p.base != nullptr);
+      if (ok1) *reinterpret_cast<uint4*>(p.out + row1 * p.ld_out + col) = ld16(p.base + row1 * p.ld_base + col, p.base != nullptr);
+    }
+    return;
+  }
+
+  // ---- first product: this warp's part of K
+  float acc[RT][4];
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+  const int steps = (p.K + 31) >> 5;
+  const int k_lo = static_cast<int>(static_cast<long long>(steps) * part / parts), k_hi = static_cast<int>(static_cast<long long>(steps) * (part + 1) / parts);
+  const __nv_bfloat16* x0 = p.in + row0 * p.ld_in;
+  const __nv_bfloat16* x1 = p.in + row1 * p.ld_in;
+  const __nv_bfloat16* down = p.down + static_cast<size_t>(tile.x) * p.r * p.K;
+  const uint32_t scratch = smem_u32(smem + (kSplits + 1) * 16 * MT * LD) + warp * 2048;
+#pragma unroll 2
+  for (int s = k_lo; s < k_hi; ++s) {
+    const int k = s * 32 + 8 * t;
+    const bool in = k < p.K;
+    const uint4 a = ld16(x0 + k, in), b = ld16(x1 + k, in);
+    if constexpr (!ACROSS) {
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        const uint4 f = ld16(down + static_cast<size_t>(8 * j + g) * p.K + k, in && (RT <= 2 || 8 * j < p.r));
+        mma16816(acc[j], a.x, b.x, a.y, b.y, f.x, f.y);
+        mma16816(acc[j], a.z, b.z, a.w, b.w, f.z, f.w);
+      }
+    } else {
+      // rows of the factor are k: lane l brings row l. Matrix i of a transposed read holds the rows with the same place
+      // among a lane's pairs, so that the products get the same k as above
+      const int kr = s * 32 + lane;
+      const uint32_t put = scratch + ((((lane >> 1) & 3) * 8 + 2 * (lane >> 3) + (lane & 1)) << 4);
+#pragma unroll
+      for (int j0 = 0; j0 < RT; j0 += 4) {
+        __syncwarp();
+#pragma unroll
+        for (int j = j0; j < (RT < j0 + 4 ? RT : j0 + 4); ++j) {
+          const uint4 f = ld16(down + static_cast<size_t>(kr) * p.r + 8 * j, kr < p.K && (RT <= 2 || 8 * j < p.r));
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(put + (j - j0) * 512), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = j0; j < (RT < j0 + 4 ? RT : j0 + 4); ++j) {
+          uint32_t f[4];
+          ldsm4t(scratch + (j - j0) * 512 + lane * 16, f);
+          mma16816(acc[j], a.x, b.x, a.y, b.y, f[0], f[1]);
+          mma16816(acc[j], a.z, b.z, a.w, b.w, f[2], f[3]);
+        }
+      }
+    }
+  }
+
+  // ---- h: sum over the warps of a row group, then over the cluster, both in order
+  float* sum = smem + kSplits * 16 * MT * LD;
+  {
+    float* mine = smem + ks * 16 * MT * LD;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      *reinterpret_cast<float2*>(mine + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(mine + r1 * LD + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
+  }
+  __syncthreads();
+  const float sc = p.scale[tile.x];
+  constexpr int kVals = 16 * MT * 8 * RT;
+  for (int i = threadIdx.x * 4; i < kVals; i += kWarps * 32 * 4) {
+    const int at = (i / (8 * RT)) * LD + i % (8 * RT);
+    float4 v = *reinterpret_cast<const float4*>(smem + at);
+#pragma unroll
+    for (int q = 1; q < kSplits; ++q) {
+      const float4 w = *reinterpret_cast<const float4*>(smem + q * 16 * MT * LD + at);
+      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    }
+    *reinterpret_cast<float4*>(sum + at) = v;
+  }
+  float* fin = smem;                                   // the cluster's sum, scaled, replaces the first partial
+  if (c > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (int i = threadIdx.x * 4; i < kVals; i += kWarps * 32 * 4) {
+      const int at = (i / (8 * RT)) * LD + i % (8 * RT);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < c; ++q) {
+        const float4 w = *reinterpret_cast<const float4*>(cl.map_shared_rank(sum, q) + at);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      *reinterpret_cast<float4*>(fin + at) = make_float4(v.x * sc, v.y * sc, v.z * sc, v.w * sc);
+    }
+    cl.sync();                                         // nobody reads a peer's sum after this
+  } else {
+    __syncthreads();
+    for (int i = threadIdx.x * 4; i < kVals; i += kWarps * 32 * 4) {
+      const int at = (i / (8 * RT)) * LD + i % (8 * RT);
+      const float4 v = *reinterpret_cast<const float4*>(sum + at);
+      *reinterpret_cast<float4*>(fin + at) = make_float4(v.x * sc, v.y * sc, v.z * sc, v.w * sc);
+    }
+    __syncthreads();
+  }
+  if (p.h != nullptr && rank_cta == 0) {
+    for (int i = threadIdx.x * 2; i < tile.z * p.r; i += kWarps * 32 * 2) {
+      const int row = i / p.r, q = i % p.r;
+      uint32_t hi, lo;
+      split2(fin[row * LD + q], fin[row * LD + q + 1], hi, lo);
+      const size_t at = static_cast<size_t>(tile.y + row) * p.r + q;
+      *reinterpret_cast<uint32_t*>(p.h + at) = hi;
+      *reinterpret_cast<uint32_t*>(p.h + static_cast<size_t>(p.T) * p.r + at) = lo;
+    }
+  }
+  if (p.out == nullptr) return;
+
+  // ---- second product: this warp's columns. Tile j of a chunk holds the columns with the same place among a lane's
+  // pairs, so a lane ends with 8 neighbouring columns of its two rows
+  uint32_t hi[KS][4], lo[KS][4];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    // ranks of the two pairs of a step: as a lane's wide load of B brings them, or in order where the factor is read across
+    const int qa = ACROSS ? 16 * s + 2 * t : RT == 1 ? 2 * t : RT == 2 ? 4 * t : (s >> 1) * 32 + 8 * t + 4 * (s & 1);
+    const int qb = ACROSS ? qa + 8 : qa + 2;
+    const float2 z = make_float2(0.f, 0.f);
+    const float2 f0 = *reinterpret_cast<const float2*>(fin + r0 * LD + qa), f1 = *reinterpret_cast<const float2*>(fin + r1 * LD + qa);
+    const float2 f2 = RT == 1 ? z : *reinterpret_cast<const float2*>(fin + r0 * LD + qb), f3 = RT == 1 ? z : *reinterpret_cast<const float2*>(fin + r1 * LD + qb);
+    split2(f0.x, f0.y, hi[s][0], lo[s][0]);
+    split2(f1.x, f1.y, hi[s][1], lo[s][1]);
+    split2(f2.x, f2.y, hi[s][2], lo[s][2]);
+    split2(f3.x, f3.y, hi[s][3], lo[s][3]);
+  }
+  const __nv_bfloat16* up = p.up + static_cast<size_t>(tile.x) * p.r * p.N;
+  for (int n = n_lo; n < n_hi; ++n) {
+    const int col = n * 32 + 8 * t;
+    const bool in = col < p.N;
+    const uint4 y0 = ld16(p.base + row0 * p.ld_base + col, in && p.base != nullptr), y1 = ld16(p.base + row1 * p.ld_base + col, in && p.base != nullptr);
+    float o[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    if constexpr (!ACROSS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int bc = n * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
+        const __nv_bfloat16* f = up + static_cast<size_t>(bc) * p.r;
+        const bool inb = bc < p.N;
+        if constexpr (RT == 1) {
+          const uint32_t b = inb ? *reinterpret_cast<const uint32_t*>(f + 2 * t) : 0u;
+          mma16816(o[j], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b, 0u);
+          mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b, 0u);
+        } else if constexpr (RT == 2) {
+          const uint2 b = inb ? *reinterpret_cast<const uint2*>(f + 4 * t) : make_uint2(0u, 0u);
+          mma16816(o[j], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b.x, b.y);
+          mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b.x, b.y);
+        } else {
+#pragma unroll
+          for (int q = 0; q < RT / 4; ++q) {
+            const uint4 b = ld16(f + 32 * q + 8 * t, inb && 32 * q + 8 * t < p.r);
+            mma16816(o[j], hi[2 * q][0], hi[2 * q][1], hi[2 * q][2], hi[2 * q][3], b.x, b.y);
+            mma16816(o[j], lo[2 * q][0], lo[2 * q][1], lo[2 * q][2], lo[2 * q][3], b.x, b.y);
+            mma16816(o[j], hi[2 * q + 1][0], hi[2 * q + 1][1], hi[2 * q + 1][2], hi[2 * q + 1][3], b.z, b.w);
+            mma16816(o[j], lo[2 * q + 1][0], lo[2 * q + 1][1], lo[2 * q + 1][2], lo[2 * q + 1][3], b.z, b.w);
+          }
+        }
+      }
+    } else {
+      // rows of the factor are ranks: 8 of them x 32 columns at a time, each lane's 4 pairs of columns into the 4 tiles
+#pragma unroll
+      for (int i0 = 0; i0 < RT; i0 += 4) {
+        __syncwarp();
+#pragma unroll
+        for (int i = i0; i < (RT < i0 + 4 ? RT : i0 + 4); ++i) {
+          const uint4 f = ld16(up + static_cast<size_t>(8 * i + g) * p.N + col, in && (RT <= 2 || 8 * i < p.r));
+          const uint32_t put = scratch + (i - i0) * 128 + lane * 4;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(put), "r"(f.x) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(put + 512), "r"(f.y) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(put + 1024), "r"(f.z) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(put + 1536), "r"(f.w) : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b[4];
+          ldsm4t(scratch + j * 512 + lane * 16, b);      // ranks 8 i0 .. 8 i0 + 31 of tile j; what RT does not fill is not used
+          mma16816(o[j], hi[i0 / 2][0], hi[i0 / 2][1], hi[i0 / 2][2], hi[i0 / 2][3], b[0], RT == 1 ? 0u : b[1]);
+          mma16816(o[j], lo[i0 / 2][0], lo[i0 / 2][1], lo[i0 / 2][2], lo[i0 / 2][3], b[0], RT == 1 ? 0u : b[1]);
+          if constexpr (RT >= 4) {
+            mma16816(o[j], hi[i0 / 2 + 1][0], hi[i0 / 2 + 1][1], hi[i0 / 2 + 1][2], hi[i0 / 2 + 1][3], b[2], b[3]);
+            mma16816(o[j], lo[i0 / 2 + 1][0], lo[i0 / 2 + 1][1], lo[i0 / 2 + 1][2], lo[i0 / 2 + 1][3], b[2], b[3]);
+          }
+        }
+      }
+    }
+    uint4 w0, w1;
+    const __nv_bfloat162* b0 = reinterpret_cast<const __nv_bfloat162*>(&y0);
+    const __nv_bfloat162* b1 = reinterpret_cast<const __nv_bfloat162*>(&y1);
+    __nv_bfloat162* v0 = reinterpret_cast<__nv_bfloat162*>(&w0);
+    __nv_bfloat162* v1 = reinterpret_cast<__nv_bfloat162*>(&w1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v0[j] = __floats2bfloat162_rn(__low2float(b0[j]) + o[j][0], __high2float(b0[j]) + o[j][1]);
+      v1[j] = __floats2bfloat162_rn(__low2float(b1[j]) + o[j][2], __high2float(b1[j]) + o[j][3]);
+    }
+    if (in && ok0) *reinterpret_cast<uint4*>(p.out + row0 * p.ld_out + col) = w0;
+    if (in && ok1) *reinterpret_cast<uint4*>(p.out + row1 * p.ld_out + col) = w1;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ gradients of the factors
+// G[rank, col] = sum over an adapter's tokens of h[t, rank] z[t, col]. A CTA owns 128 columns of one adapter, its cluster
+// splits the adapter's tokens; a warp owns 16 columns and all ranks. Tokens are the contracted index, so both operands are
+// read across (transposed reads of shared memory) from tiles of 32 tokens that asynchronous copies bring in kStages deep.
+// h is the two bf16 numbers that lora_apply_kernel stored; sums are fp32, partial sums of the cluster are added in order.
+struct GradArgs {
+  const __nv_bfloat16* h;     // [2, T, r], plan's order
+  const __nv_bfloat16* z;     // [T, C] rows by token
+  __nv_bfloat16* out;         // [E, r, C], or by columns [E, C, r]
+  const int* perm;
+  const int* offsets;
+  long long ld_z;
+  int T, C, r, by_cols;
+};
+constexpr int kTok = 32, kCols = 128, kStages = 4;
+constexpr int kZRow = kCols * 2 + 16;                  // bytes a row in shared memory: 16 more spread the transposed reads
+
+template <int RT>
+constexpr int grad_stage() {
+  return kTok * kZRow + 2 * kTok * (8 * RT * 2 + 16);
+}
+template <int RT>
+constexpr int grad_smem() {
+  const int ring = kStages * grad_stage<RT>(), sums = kCols * (8 * RT + 1) * 4;
+  return ring > sums ? ring : sums;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+template <int RT>
+__global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ GradArgs p) {
+  constexpr int kHRow = 8 * RT * 2 + 16;
+  extern __shared__ __align__(16) uint8_t ring[];
+  const int c = gridDim.x, rank_cta = blockIdx.x, a = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col0 = blockIdx.y * kCols;
+  const int t0 = p.offsets[a], t1 = p.offsets[a + 1];
+  const int tiles = (t1 - t0 + kTok - 1) / kTok;
+  const int lo = static_cast<int>(static_cast<long long>(tiles) * rank_cta / c), hi = static_cast<int>(static_cast<long long>(tiles) * (rank_cta + 1) / c);
+  const uint32_t base = smem_u32(ring);
+  constexpr int kHVec = RT;                            // 16-byte pieces a row of h
+  auto load = [&](int tile) {
+    if (tile < hi) {
+      const uint32_t st = base + (tile % kStages) * grad_stage<RT>();
+      const int first = t0 + tile * kTok;
+      for (int i = threadIdx.x; i < kTok * (kCols / 8); i += 256) {
+        const int row = i / (kCols / 8), v = i % (kCols / 8);
+        const bool ok = first + row < t1 && col0 + v * 8 < p.C;
+        const __nv_bfloat16* src = p.z;
+        if (ok) src += static_cast<long long>(p.perm[first + row]) * p.ld_z + col0 + v * 8;
+        cp16(st + row * kZRow + v * 16, src, ok);
+      }
+      for (int i = threadIdx.x; i < 2 * kTok * kHVec; i += 256) {
+        const int part = i / (kTok * kHVec), row = i / kHVec % kTok, v = i % kHVec;
+        const bool ok = first + row < t1 && v * 8 < p.r;
+        const __nv_bfloat16* src = p.h;
+        if (ok) src += (static_cast<size_t>(part) * p.T + first + row) * p.r + v * 8;
+        cp16(st + kTok * kZRow + (part * kTok + row) * kHRow + v * 16, src, ok);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float acc[RT][4];
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(lo + s);
+  for (int tile = lo; tile < hi; ++tile) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();                                   // the tile has landed, and everybody is done with the one before
+    load(tile + kStages - 1);
+    const uint32_t st = base + (tile % kStages) * grad_stage<RT>();
+    const uint32_t hs = st + kTok * kZRow;
+#pragma unroll
+    for (int k = 0; k < kTok; k += 16) {
+      // columns are the rows of the product: matrices (tokens k..k+7 | k+8..k+15) x (columns 0..7 | 8..15)
+      uint32_t za[4];
+      ldsm4t(st + (k + (lane & 7) + 8 * (lane >> 4)) * kZRow + (warp * 16 + 8 * ((lane >> 3) & 1)) * 2, za);
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        uint32_t b[4];                                 // (hi, lo) x (tokens k..k+7 | k+8..k+15)
+        ldsm4t(hs + ((lane >> 4) * kTok + k + (lane & 7) + 8 * ((lane >> 3) & 1)) * kHRow + j * 16, b);
+        mma16816(acc[j], za[0], za[1], za[2], za[3], b[0], b[1]);
+        mma16816(acc[j], za[0], za[1], za[2], za[3], b[2], b[3]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  // sums of this CTA: [column][rank]
+  constexpr int LD = 8 * RT + 1;
+  float* mine = reinterpret_cast<float*>(ring);
+  {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      float* w = mine + (warp * 16 + g) * LD + 8 * j + 2 * t;
+      w[0] = acc[j][0], w[1] = acc[j][1];
+      w[8 * LD] = acc[j][2], w[8 * LD + 1] = acc[j][3];
+    }
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  const int cols = min(kCols, p.C - col0);
+  __nv_bfloat16* out = p.out + static_cast<size_t>(a) * p.r * p.C;
+  // the cluster's CTAs share the output's elements
+  for (int i = rank_cta * 256 + threadIdx.x; i < cols * p.r; i += c * 256) {
+    const int col = p.by_cols ? i / p.r : i % cols, q = p.by_cols ? i % p.r : i / cols;
+    float v = 0.f;
+    for (int k = 0; k < c; ++k) v += cl.map_shared_rank(mine, k)[col * LD + q];
+    out[p.by_cols ? static_cast<size_t>(col0 + col) * p.r + q : static_cast<size_t>(q) * p.C + col0 + col] = __float2bfloat16_rn(v);
+  }
+  cl.sync();
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+template <typename Args>
+int launch_cluster(void (*kern)(Args), const Args& args, dim3 grid, int cluster, int smem, cudaStream_t s) {
+  if (smem > 48 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  IX_CUDA(cudaLaunchKernelEx(&cfg, kern, args));
+  return 0;
+}
+
+template <int RT, int MT>
+int apply_across(const ApplyArgs& a, int across, dim3 grid, cudaStream_t s) {
+  if (across) return launch_cluster(lora_apply_kernel<RT, MT, true>, a, grid, grid.x, apply_smem<RT, MT>(true), s);
+  return launch_cluster(lora_apply_kernel<RT, MT, false>, a, grid, grid.x, apply_smem<RT, MT>(false), s);
+}
+template <int RT>
+int apply_tile(const ApplyArgs& a, int large, int across, dim3 grid, cudaStream_t s) {
+  return large ? apply_across<RT, kLarge / 16>(a, across, grid, s) : apply_across<RT, 1>(a, across, grid, s);
+}
+
+inline int bound_tiles(int T, int E, int size) {
+  const int groups = E + 1 < T ? E + 1 : T;
+  const long long b = static_cast<long long>(T) / size + groups;
+  return static_cast<int>(b < T ? b : T);
+}
+
+}  // namespace
+
+IX_API int ix_lora_max_adapters() { return kMaxAdapters; }
+// Upper bound of the number of tiles of the small (large = 0) or large size: the tile lists hold that many int4.
+IX_API int ix_lora_max_tiles(int T, int E, int large) { return bound_tiles(T, E, large ? kLarge : kSmall); }
+
+// ids int32 [T]; perm int32 [T]; offsets int32 [E + 2]; tiles int4; n_tiles int32 [2] (small, large).
+IX_API int ix_lora_plan(const void* ids, int T, int E, void* perm, void* offsets, void* tiles_small, void* tiles_large, void* n_tiles, void* stream) {
+  if (T <= 0) return 0;
+  if (E < 1 || E > kMaxAdapters) return ixh::fail(ixh::IX_EARG, "lora: 1 to %d adapters, not %d", kMaxAdapters, E);
+  // warps: as many as the counters leave room for (48 KB without an opt-in)
+  int warps = 32;
+  while (warps > 1 && (warps + 1) * (E + 1) * 4 > 34 * 1024) warps >>= 1;
+  lora_plan_kernel<<<1, warps * 32, (warps + 1) * (E + 1) * 4, reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const int*>(ids), T, E, static_cast<int*>(perm), static_cast<int*>(offsets), static_cast<int4*>(tiles_small),
+      static_cast<int4*>(tiles_large), static_cast<int*>(n_tiles));
+  IX_CUDA(cudaGetLastError());
+  return 0;
+}
+
+// across = 0: out = base + s (in down^T) up^T, down [E, r, K], up [E, N, r]. across = 1: the same with down [E, K, r] and
+// up [E, r, N]. base null: zero; out null: only h. h (may be null): bf16 [2, T, r]. All leading dimensions multiples of 8.
+IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long long ld_base, void* out, long long ld_out, const void* down,
+                         const void* up, const void* scale, const void* perm, const void* tiles_small, const void* tiles_large, const void* n_tiles,
+                         void* h, int T, int K, int N, int r, int E, int across, void* stream) {
+  if (T <= 0) return 0;
+  if (r < 8 || r > kMaxRank || r % 8) return ixh::fail(ixh::IX_EARG, "lora: rank %d is not a multiple of 8 up to %d", r, kMaxRank);
+  if (K < 8 || N < 8 || K % 8 || N % 8) return ixh::fail(ixh::IX_EARG, "lora: widths %d and %d must be multiples of 8", K, N);
+  if (ld_in % 8 || ld_base % 8 || ld_out % 8) return ixh::fail(ixh::IX_EARG, "lora: row strides must be multiples of 8");
+  ApplyArgs a;
+  a.in = static_cast<const __nv_bfloat16*>(in);
+  a.base = static_cast<const __nv_bfloat16*>(base);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.down = static_cast<const __nv_bfloat16*>(down);
+  a.up = static_cast<const __nv_bfloat16*>(up);
+  a.scale = static_cast<const float*>(scale);
+  a.perm = static_cast<const int*>(perm);
+  a.h = static_cast<__nv_bfloat16*>(h);
+  a.ld_in = ld_in, a.ld_base = ld_base, a.ld_out = ld_out;
+  a.T = T, a.K = K, a.N = N, a.r = r;
+  // large tiles where adapters have many tokens: they read the factors a quarter as often
+  const int large = T / E >= 48;
+  a.tiles = static_cast<const int4*>(large ? tiles_large : tiles_small);
+  a.n_tiles = static_cast<const int*>(n_tiles) + large;
+  const int tiles = bound_tiles(T, E, large ? kLarge : kSmall);
+  if (tiles > 65535) return ixh::fail(ixh::IX_ESIZE, "lora: %d tokens of %d adapters make more than 65535 tiles", T, E);
+  // CTAs a tile: until the card has three a multiprocessor, but not beyond one step of 32 a warp
+  int c = 1;
+  const int widest = (K > N ? K : N) / 32;
+  while (c < 8 && tiles * c < 148 * 3 && widest > c * (large ? 2 : 8)) c *= 2;
+  const dim3 grid(c, tiles);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (r <= 8) return apply_tile<1>(a, large, across, grid, s);
+  if (r <= 16) return apply_tile<2>(a, large, across, grid, s);
+  if (r <= 32) return apply_tile<4>(a, large, across, grid, s);
+  if (r <= 64) return apply_tile<8>(a, large, across, grid, s);
+  return apply_tile<16>(a, large, across, grid, s);
+}
+
+// out[a] = sum over the adapter's tokens of h[t]^T z[t]: bf16 [E, r, C], or by columns [E, C, r]; zero without tokens.
+IX_API int ix_lora_grad(const void* h, const void* z, long long ld_z, void* out, const void* perm, const void* offsets, int T, int C, int r, int E,
+                        int by_cols, void* stream) {
+  if (r < 8 || r > kMaxRank || r % 8) return ixh::fail(ixh::IX_EARG, "lora: rank %d is not a multiple of 8 up to %d", r, kMaxRank);
+  if (C < 8 || C % 8 || ld_z % 8) return ixh::fail(ixh::IX_EARG, "lora: width %d and its row stride must be multiples of 8", C);
+  GradArgs a;
+  a.h = static_cast<const __nv_bfloat16*>(h);
+  a.z = static_cast<const __nv_bfloat16*>(z);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.perm = static_cast<const int*>(perm);
+  a.offsets = static_cast<const int*>(offsets);
+  a.ld_z = ld_z;
+  a.T = T, a.C = C, a.r = r, a.by_cols = by_cols;
+  const int tiles = (C + kCols - 1) / kCols;
+  if (T <= 0) {
+    IX_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(E) * r * C * 2, reinterpret_cast<cudaStream_t>(stream)));
+    return 0;
+  }
+  // CTAs an adapter's columns: until the card has three a multiprocessor, but not beyond four tiles of tokens each
+  int c = 1;
+  while (c < 8 && tiles * E * c < 148 * 3 && T > c * 4 * kTok) c *= 2;
+  const dim3 grid(c, tiles, E);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (r <= 8) return launch_cluster(lora_grad_kernel<1>, a, grid, c, grad_smem<1>(), s);
+  if (r <= 16) return launch_cluster(lora_grad_kernel<2>, a, grid, c, grad_smem<2>(), s);
+  if (r <= 32) return launch_cluster(lora_grad_kernel<4>, a, grid, c, grad_smem<4>(), s);
+  if (r <= 64) return launch_cluster(lora_grad_kernel<8>, a, grid, c, grad_smem<8>(), s);
+  return launch_cluster(lora_grad_kernel<16>, a, grid, c, grad_smem<16>(), s);
+}

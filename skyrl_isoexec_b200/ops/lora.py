@@ -1,0 +1,240 @@
+"""Low-rank adapters of many requests at once beside a shared projection: ``y[t] + s_a (x[t] A_a^T) B_a^T`` with the adapter
+``a`` of token ``t``, and the gradients of ``x``, ``A`` and ``B``. CUDA tensors (bf16) go to csrc/lora.cu, CPU tensors to
+torch in fp32 with the same roundings. ``train/lora.py`` merges ONE adapter into the weights instead; there rollouts keep the
+trainer's bits, here a batch may hold a different adapter in every row.
+
+An adapter bank is two tensors, ``A [E, r, K]`` and ``B [E, N, r]``, with ``scale [E]`` in fp32 (``alpha / rank``). Adapters of
+different ranks share a bank when the smaller ones are filled up with zero rows of ``A`` and zero columns of ``B``
+(``pad_rank``): the result does not change."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from . import functional as F
+
+MAX_RANK = 128
+
+
+class LoraPlan:
+    """The tokens of a batch grouped by adapter. ``ids``: integer [T], the adapter of every token; a number outside
+    ``[0, num_adapters)`` means none. Built on the device in one launch without a look at the ids on the host (so a plan can
+    be captured, and is built again by a replay); one plan serves every projection of every layer of the batch."""
+
+    def __init__(self, ids: torch.Tensor, num_adapters: int):
+        if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"LoraPlan: ids are a flat int32 or int64 tensor, not {tuple(ids.shape)} {ids.dtype}")
+        if num_adapters < 1:
+            raise ValueError("LoraPlan: at least one adapter")
+        self.T, self.E, self.device = ids.shape[0], int(num_adapters), ids.device
+        if not ids.is_cuda:
+            self.ids = ids.clone()
+            return
+        L = _native.lib()
+        if self.E > L.ix_lora_max_adapters():
+            raise ValueError(f"LoraPlan: at most {L.ix_lora_max_adapters()} adapters in a batch, not {self.E}")
+        if ids.dtype == torch.int64:                # a number that 32 bits would wrap into the range stays outside
+            ids = torch.where((ids < 0) | (ids >= self.E), -1, ids)
+        ids = ids.to(torch.int32).contiguous()
+        small, large = (L.ix_lora_max_tiles(self.T, self.E, k) for k in (0, 1))
+        buf = torch.empty(4 * small + 4 * large + self.T + self.E + 2 + 2, dtype=torch.int32, device=ids.device)
+        self.tiles_small, self.tiles_large, self.perm, self.offsets, self.n_tiles = buf.split(
+            [4 * small, 4 * large, self.T, self.E + 2, 2])
+        with torch.cuda.device(ids.device):
+            _native.check(L.ix_lora_plan(ids.data_ptr(), self.T, self.E, self.perm.data_ptr(), self.offsets.data_ptr(),
+                                         self.tiles_small.data_ptr(), self.tiles_large.data_ptr(), self.n_tiles.data_ptr(), _native.stream()),
+                          "ix_lora_plan")
+
+
+def pad_rank(A: torch.Tensor, B: torch.Tensor, rank: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """One adapter's ``A [r, K]`` and ``B [N, r]`` filled up with zeros to ``rank``."""
+    r = A.shape[0]
+    if A.dim() != 2 or B.dim() != 2 or B.shape[1] != r or rank < r:
+        raise ValueError(f"pad_rank: A {tuple(A.shape)} and B {tuple(B.shape)} do not fit rank {rank}")
+    return torch.nn.functional.pad(A, (0, 0, 0, rank - r)), torch.nn.functional.pad(B, (0, rank - r))
+
+
+def _check(y, x, A, B, scale, plan) -> None:
+    if A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
+        raise ValueError(f"lora: factors are A [E, r, K] and B [E, N, r], not {tuple(A.shape)} and {tuple(B.shape)}")
+    E, r, K = A.shape
+    N = B.shape[1]
+    if x.shape[-1] != K or (y is not None and (y.shape[-1] != N or y.shape[:-1] != x.shape[:-1])):
+        raise ValueError(f"lora: x {tuple(x.shape)} and y {None if y is None else tuple(y.shape)} do not fit factors of widths {K} and {N}")
+    if plan.E != E or plan.T != x.numel() // K:
+        raise ValueError(f"lora: the plan is for {plan.T} tokens of {plan.E} adapters, x has {x.numel() // K} and the bank {E}")
+    if scale.shape != (E,) or scale.dtype != torch.float32:
+        raise ValueError(f"lora: scale is fp32 [{E}], not {tuple(scale.shape)} {scale.dtype}")
+    if scale.requires_grad:
+        raise ValueError("lora: scale is a constant, it has no gradient")
+    ts = [t for t in (y, x, A, B) if t is not None]
+    if any(t.device != plan.device for t in ts) or scale.device != plan.device:
+        raise ValueError("lora: all tensors and the plan are on one device")
+    if any(t.dtype != x.dtype for t in ts):
+        raise ValueError("lora: x, y, A and B have one type")
+    if x.is_cuda:
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"lora: on a GPU the tensors are bf16, not {x.dtype}")
+        if r % 8 or r > MAX_RANK or K % 8 or N % 8:
+            raise ValueError(f"lora: rank {r} (a multiple of 8 up to {MAX_RANK}: pad_rank) and widths {K}, {N} (multiples of 8)")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[T, width] with unit inner stride, rows on 16-byte boundaries."""
+    t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] and (t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _factor(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _apply(x, base, out, down, up, scale, plan, across, want_h):
+    """csrc/lora.cu::ix_lora_apply on prepared operands; returns h [2, T, r] in the plan's order if wanted."""
+    T, K = x.shape
+    E = plan.E
+    r, N = (down.shape[1], up.shape[1]) if not across else (down.shape[2], up.shape[2])
+    h = torch.empty(2, T, r, dtype=torch.bfloat16, device=x.device) if want_h else None
+    if T == 0:
+        return h
+    _native.check(
+        _native.lib().ix_lora_apply(x.data_ptr(), x.stride(0), _native.ptr(base), base.stride(0) if base is not None else 0, _native.ptr(out),
+                                    out.stride(0) if out is not None else 0, down.data_ptr(), up.data_ptr(), scale.data_ptr(),
+                                    plan.perm.data_ptr(), plan.tiles_small.data_ptr(), plan.tiles_large.data_ptr(), plan.n_tiles.data_ptr(),
+                                    _native.ptr(h), T, K, N, r, E, int(across), _native.stream()),
+        "ix_lora_apply")
+    return h
+
+
+def _factor_grad(h, z, like, plan, by_cols):
+    out = torch.empty_like(like, memory_format=torch.contiguous_format)
+    r, C = (like.shape[2], like.shape[1]) if by_cols else (like.shape[1], like.shape[2])
+    _native.check(
+        _native.lib().ix_lora_grad(h.data_ptr(), z.data_ptr(), z.stride(0), out.data_ptr(), plan.perm.data_ptr(), plan.offsets.data_ptr(),
+                                   plan.T, C, r, plan.E, int(by_cols), _native.stream()),
+        "ix_lora_grad")
+    return out
+
+
+def _cpu_h(x, A, scale, plan):
+    """s (x A^T) of every token with its own adapter, fp32 [T, r]; zero rows without one."""
+    h = torch.zeros(x.shape[0], A.shape[1])
+    for a in range(plan.E):
+        rows = (plan.ids == a).nonzero()[:, 0]
+        h[rows] = scale[a] * (x[rows].float() @ A[a].float().t())
+    return h
+
+
+def _cpu_up(h, B, plan):
+    out = torch.zeros(h.shape[0], B.shape[1])
+    for a in range(plan.E):
+        rows = (plan.ids == a).nonzero()[:, 0]
+        out[rows] = h[rows] @ B[a].float().t()
+    return out
+
+
+def _cpu_grad(h, z, plan):
+    return torch.stack([h[plan.ids == a].t() @ z[plan.ids == a].float() for a in range(plan.E)])
+
+
+def _forward(y, x, A, B, scale, plan, inplace: bool, want_h: bool):
+    """(out, h) on rows; ``inplace``: out is y."""
+    if x.is_cuda:
+        with torch.cuda.device(x.device):
+            out = y if inplace else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+            return out, _apply(x, y, out, A, B, scale, plan, False, want_h)
+    h = _cpu_h(x, A, scale, plan)
+    hit = ((plan.ids >= 0) & (plan.ids < plan.E))[:, None]
+    out = torch.where(hit, (y.float() + _cpu_up(h, B, plan)).to(y.dtype), y)
+    return (y.copy_(out) if inplace else out), h
+
+
+def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, need_b: bool):
+    """(dx, dA, dB); ``base``: the other part of dx, added to in place."""
+    dx = dA = dB = None
+    if x.is_cuda:
+        with torch.cuda.device(x.device):
+            g = None
+            if need_x or need_a:
+                dx = None if not need_x else base if base is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                g = _apply(dy, base if need_x else None, dx, B, A, scale, plan, True, need_a)
+            if need_a:
+                dA = _factor_grad(g, x, A, plan, False)
+            if need_b:
+                dB = _factor_grad(h, dy, B, plan, True)
+        return dx, dA, dB
+    g = _cpu_h(dy, B.transpose(1, 2), scale, plan)
+    if need_x:
+        dx = _cpu_up(g, A.transpose(1, 2), plan)
+        dx = (dx if base is None else base.float() + dx).to(x.dtype)
+    if need_a:
+        dA = _cpu_grad(g, x, plan).to(A.dtype)
+    if need_b:
+        dB = _cpu_grad(h, dy, plan).transpose(1, 2).contiguous().to(B.dtype)
+    return dx, dA, dB
+
+
+class _LoraAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, A, B, scale, plan):
+        x2, A2, B2 = _rows(x), _factor(A), _factor(B)
+        out, h = _forward(_rows(y), x2, A2, B2, scale, plan, False, ctx.needs_input_grad[3])
+        ctx.save_for_backward(x2, A2, B2, scale, h)
+        ctx.plan, ctx.xshape = plan, x.shape
+        return out.view(y.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, A, B, scale, h = ctx.saved_tensors
+        ny, nx, na, nb = ctx.needs_input_grad[:4]
+        dx, dA, dB = _backward(_rows(dout), x, A, B, scale, h, ctx.plan, None, nx, na, nb)
+        return (dout if ny else None), (dx.view(ctx.xshape) if nx else None), dA, dB, None, None
+
+
+class _LoraLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, A, B, scale, plan):
+        x2, A2, B2 = _rows(x), _factor(A), _factor(B)
+        out, h = _forward(F.gemm_nt(x2, w), x2, A2, B2, scale, plan, True, ctx.needs_input_grad[3])
+        ctx.save_for_backward(x2, w, A2, B2, scale, h)
+        ctx.plan, ctx.xshape = plan, x.shape
+        return out.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, w, A, B, scale, h = ctx.saved_tensors
+        nx, nw, na, nb = ctx.needs_input_grad[:4]
+        dy = _rows(dout)
+        base = F.gemm_nn(dy, w) if nx else None
+        dx, dA, dB = _backward(dy, x, A, B, scale, h, ctx.plan, base, nx, na, nb)
+        dw = F.gemm_tn(dy, x) if nw else None
+        return (dx.view(ctx.xshape) if nx else None), dw, dA, dB, None, None
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scale: torch.Tensor, plan: LoraPlan) -> torch.Tensor:
+    """``y + s_a (x A_a^T) B_a^T`` for every token's own adapter: x [..., K], y [..., N], A [E, r, K], B [E, N, r], scale [E].
+    One rounding, of the result; a token without an adapter gets y's bits. Differentiable in y, x, A and B."""
+    _check(y, x, A, B, scale, plan)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, A, B)):
+        return _LoraAdd.apply(y, x, A, B, scale, plan)
+    return _forward(_rows(y), _rows(x), _factor(A), _factor(B), scale, plan, False, False)[0].view(y.shape)
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scale: torch.Tensor, plan: LoraPlan) -> torch.Tensor:
+    """``F.linear(x, w)`` with the tokens' adapters added into its result in place (``lora_add`` without the second buffer).
+    Differentiable in x, w, A and B; a frozen ``w`` costs no product in the backward."""
+    _check(None, x, A, B, scale, plan)
+    if w.dim() != 2 or w.shape != (B.shape[1], A.shape[2]) or w.dtype != x.dtype or w.device != x.device:
+        raise ValueError(f"lora: w {tuple(w.shape)} {w.dtype} does not fit factors of widths {A.shape[2]} and {B.shape[1]}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w, A, B)):
+        return _LoraLinear.apply(x, w, A, B, scale, plan)
+    x2 = _rows(x)
+    return _forward(F.gemm_nt(x2, w), x2, _factor(A), _factor(B), scale, plan, True, False)[0].view(*x.shape[:-1], w.shape[0])
