@@ -142,18 +142,17 @@ struct ApplyArgs {
 };
 
 constexpr int kWarps = 8;
-// shared memory: partial sums [kWarps / MT][16 MT][8 RT + 4] fp32, their sum [16 MT][8 RT + 4], a warp's 2 KB for factors
-// that are read across
-template <int RT, int MT>
+// shared memory: partial sums [kWarps][16][8 RT + 4] fp32, their sum [16][8 RT + 4], a warp's 2 KB for factors that are
+// read across
+template <int RT>
 constexpr int apply_smem(bool across) {
-  return (kWarps / MT + 1) * 16 * MT * (8 * RT + 4) * 4 + (across ? kWarps * 2048 : 0);
+  return (kWarps + 1) * 16 * (8 * RT + 4) * 4 + (across ? kWarps * 2048 : 0);
 }
 
-// One tile of tokens. MT: 16-row groups of the tile; RT: rank in groups of 8 (r <= 8 RT); ACROSS: factors stored with the
-// contracted index outermost for the first product and innermost for the second (the backward).
-template <int RT, int MT, bool ACROSS>
+// Small tiles: 16 tokens of one adapter. RT: rank in groups of 8 (r <= 8 RT); ACROSS: factors stored with the contracted
+// index outermost for the first product and innermost for the second (the backward).
+template <int RT, bool ACROSS>
 __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_constant__ ApplyArgs p) {
-  constexpr int kSplits = kWarps / MT;                 // warps that share a 16-row group
   constexpr int LD = 8 * RT + 4;                       // floats a row of h
   constexpr int KS = RT < 2 ? 1 : RT / 2;              // depth-16 steps over the rank
   extern __shared__ __align__(16) float smem[];
@@ -161,9 +160,8 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
   const int4 tile = p.tiles[blockIdx.y];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int c = gridDim.x, rank_cta = blockIdx.x;
-  const int mt = warp % MT, ks = warp / MT;
-  const int parts = kSplits * c, part = rank_cta * kSplits + ks;
-  const int r0 = mt * 16 + g, r1 = r0 + 8;             // rows of the tile held by this lane
+  const int parts = kWarps * c, part = rank_cta * kWarps + warp;
+  const int r0 = g, r1 = r0 + 8;             // rows of the tile held by this lane
   const bool ok0 = r0 < tile.z, ok1 = r1 < tile.z;
   const long long row0 = p.perm[tile.y + (ok0 ? r0 : 0)], row1 = p.perm[tile.y + (ok1 ? r1 : 0)];
   const int chunks = (p.N + 31) >> 5;
@@ -191,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
   const __nv_bfloat16* x0 = p.in + row0 * p.ld_in;
   const __nv_bfloat16* x1 = p.in + row1 * p.ld_in;
   const __nv_bfloat16* down = p.down + static_cast<size_t>(tile.x) * p.r * p.K;
-  const uint32_t scratch = smem_u32(smem + (kSplits + 1) * 16 * MT * LD) + warp * 2048;
+  const uint32_t scratch = smem_u32(smem + (kWarps + 1) * 16 * LD) + warp * 2048;
 #pragma unroll 2
   for (int s = k_lo; s < k_hi; ++s) {
     const int k = s * 32 + 8 * t;
@@ -229,10 +227,10 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
     }
   }
 
-  // ---- h: sum over the warps of a row group, then over the cluster, both in order
-  float* sum = smem + kSplits * 16 * MT * LD;
+  // ---- h: sum over the warps, then over the cluster, both in order
+  float* sum = smem + kWarps * 16 * LD;
   {
-    float* mine = smem + ks * 16 * MT * LD;
+    float* mine = smem + warp * 16 * LD;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       *reinterpret_cast<float2*>(mine + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
@@ -241,13 +239,13 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
   }
   __syncthreads();
   const float sc = p.scale[tile.x];
-  constexpr int kVals = 16 * MT * 8 * RT;
+  constexpr int kVals = 16 * 8 * RT;
   for (int i = threadIdx.x * 4; i < kVals; i += kWarps * 32 * 4) {
     const int at = (i / (8 * RT)) * LD + i % (8 * RT);
     float4 v = *reinterpret_cast<const float4*>(smem + at);
 #pragma unroll
-    for (int q = 1; q < kSplits; ++q) {
-      const float4 w = *reinterpret_cast<const float4*>(smem + q * 16 * MT * LD + at);
+    for (int q = 1; q < kWarps; ++q) {
+      const float4 w = *reinterpret_cast<const float4*>(smem + q * 16 * LD + at);
       v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
     }
     *reinterpret_cast<float4*>(sum + at) = v;
@@ -381,11 +379,291 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
   }
 }
 
+// ------------------------------------------------------------------------------------------------ large tiles
+// 64 tokens of one adapter a cluster, for batches whose adapters have many tokens. What the small kernel asks for and waits
+// for, this one keeps in flight: a ring of kRing stages that asynchronous copies fill, 64 of K (or of N) by the tile's 64
+// rows and the factor's part, goes on through both products, so the columns' first stages are under way while the cluster
+// adds up h. Warp (m, f) owns 16 rows and one half of a stage. A stage is stored in 16-byte pieces whose place within the
+// row is xored with the row's number: reads of 8 rows at once meet 8 different bank groups.
+constexpr int kRing = 4;
+
+template <int RT>
+constexpr int tile_stage() {
+  return 64 * 128 + 64 * 16 * RT;
+}
+template <int RT>
+constexpr int tile_smem() {
+  return kRing * tile_stage<RT>() + 2 * 64 * (8 * RT + 4) * 4;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// byte of a 16-byte piece: rows of 8 pieces (64 numbers), or of RT pieces (the rank)
+__device__ __forceinline__ uint32_t wide_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+template <int RT>
+__device__ __forceinline__ uint32_t narrow_at(int row, int piece) {
+  const int x = RT >= 8 ? row & 7 : RT == 4 ? (row >> 1) & 3 : RT == 2 ? (row >> 2) & 1 : 0;
+  return row * 16 * RT + ((piece ^ x) << 4);
+}
+
+template <int RT, bool ACROSS>
+__global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ ApplyArgs p) {
+  constexpr int LD = 8 * RT + 4;
+  constexpr int KS = RT < 2 ? 1 : RT / 2;
+  extern __shared__ __align__(128) uint8_t raw[];
+  if (blockIdx.y >= p.n_tiles[0]) return;              // the same for the whole cluster
+  const int4 tile = p.tiles[blockIdx.y];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int c = gridDim.x, rank_cta = blockIdx.x;
+  const int mt = warp & 3, hf = warp >> 2;
+  const int n_all = (p.N + 63) >> 6, k_all = (p.K + 63) >> 6;
+  const int n_lo = static_cast<int>(static_cast<long long>(n_all) * rank_cta / c), n_hi = static_cast<int>(static_cast<long long>(n_all) * (rank_cta + 1) / c);
+  const int k_lo = static_cast<int>(static_cast<long long>(k_all) * rank_cta / c), k_hi = static_cast<int>(static_cast<long long>(k_all) * (rank_cta + 1) / c);
+  // rows that this thread copies (piece ch of each), and rows that it stores
+  const int ra = tid >> 3, rb = ra + 32, ch = tid & 7;
+  const bool oka = ra < tile.z, okb = rb < tile.z;
+  const long long rowa = p.perm[tile.y + (oka ? ra : 0)], rowb = p.perm[tile.y + (okb ? rb : 0)];
+  if (tile.x < 0) {                                    // no adapter: the base alone
+    if (p.out == nullptr || p.out == p.base) return;
+    for (int n = n_lo; n < n_hi; ++n) {
+      const int col = n * 64 + ch * 8;
+      if (col >= p.N) break;
+      if (oka) *reinterpret_cast<uint4*>(p.out + rowa * p.ld_out + col) = ld16(p.base + rowa * p.ld_base + col, p.base != nullptr);
+      if (okb) *reinterpret_cast<uint4*>(p.out + rowb * p.ld_out + col) = ld16(p.base + rowb * p.ld_base + col, p.base != nullptr);
+    }
+    return;
+  }
+  const uint32_t ring = smem_u32(raw);
+  float* hsum = reinterpret_cast<float*>(raw + kRing * tile_stage<RT>());
+  float* hfin = hsum + 64 * LD;
+  const int nk = k_hi - k_lo, total = nk + (p.out != nullptr ? n_hi - n_lo : 0);
+  const __nv_bfloat16* down = p.down + static_cast<size_t>(tile.x) * p.r * p.K;
+  const __nv_bfloat16* up = p.up + static_cast<size_t>(tile.x) * p.r * p.N;
+  auto wide = [&](uint32_t dst, const __nv_bfloat16* f, int width, int at) {     // rows: ranks
+#pragma unroll
+    for (int i = tid; i < 64 * RT; i += 256) {
+      const int row = i >> 3, v = i & 7;
+      const bool ok = row < p.r && at + v * 8 < width;
+      cp16(dst + wide_at(row, v), ok ? f + static_cast<size_t>(row) * width + at + v * 8 : f, ok);
+    }
+  };
+  auto narrow = [&](uint32_t dst, const __nv_bfloat16* f, int width, int at) {   // rows: K or N
+#pragma unroll
+    for (int i = tid; i < 64 * RT; i += 256) {
+      const int row = i / RT, v = i % RT;
+      const bool ok = at + row < width && v * 8 < p.r;
+      cp16(dst + narrow_at<RT>(row, v), ok ? f + static_cast<size_t>(at + row) * p.r + v * 8 : f, ok);
+    }
+  };
+  auto load = [&](int i) {
+    if (i < total) {
+      const uint32_t st = ring + (i % kRing) * tile_stage<RT>();
+      if (i < nk) {
+        const int k = (k_lo + i) * 64;
+        const bool in = k + ch * 8 < p.K;
+        cp16(st + wide_at(ra, ch), in ? p.in + rowa * p.ld_in + k + ch * 8 : p.in, in && oka);
+        cp16(st + wide_at(rb, ch), in ? p.in + rowb * p.ld_in + k + ch * 8 : p.in, in && okb);
+        if constexpr (ACROSS) narrow(st + 8192, down, p.K, k);
+        else wide(st + 8192, down, p.K, k);
+      } else {
+        const int n = (n_lo + i - nk) * 64;
+        const bool in = n + ch * 8 < p.N;
+        if (p.base != nullptr) {
+          cp16(st + wide_at(ra, ch), in ? p.base + rowa * p.ld_base + n + ch * 8 : p.base, in && oka);
+          cp16(st + wide_at(rb, ch), in ? p.base + rowb * p.ld_base + n + ch * 8 : p.base, in && okb);
+        }
+        if constexpr (ACROSS) wide(st + 8192, up, p.N, n);
+        else narrow(st + 8192, up, p.N, n);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) load(i);
+
+  // ---- first product
+  float acc[RT][4];
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+  const int l8 = lane & 7, lm = lane >> 3;             // row and matrix that this lane's address is for
+  for (int i = 0; i < nk; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    __syncthreads();                                   // the stage has landed, and everybody is done with the one before
+    load(i + kRing - 1);
+    const uint32_t st = ring + (i % kRing) * tile_stage<RT>(), fs = st + 8192;
+    uint32_t a[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) ldsm4(st + wide_at(mt * 16 + l8 + 8 * (lm & 1), hf * 4 + 2 * s + (lm >> 1)), a[s]);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      uint32_t b[4];
+      if constexpr (ACROSS) ldsm4t(fs + narrow_at<RT>(hf * 32 + lm * 8 + l8, j), b);
+      else ldsm4(fs + wide_at(j * 8 + l8, hf * 4 + lm), b);
+      mma16816(acc[j], a[0][0], a[0][1], a[0][2], a[0][3], b[0], b[1]);
+      mma16816(acc[j], a[1][0], a[1][1], a[1][2], a[1][3], b[2], b[3]);
+    }
+  }
+
+  // ---- h: the two halves, then the cluster in order: each CTA adds up its share of the rows and hands it to all
+  const int r0 = mt * 16 + g, r1 = r0 + 8;
+  if (hf == 1) {
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      *reinterpret_cast<float2*>(hfin + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(hfin + r1 * LD + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
+  }
+  __syncthreads();
+  if (hf == 0) {
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      const float2 u = *reinterpret_cast<const float2*>(hfin + r0 * LD + 8 * j + 2 * t), v = *reinterpret_cast<const float2*>(hfin + r1 * LD + 8 * j + 2 * t);
+      *reinterpret_cast<float2*>(hsum + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0] + u.x, acc[j][1] + u.y);
+      *reinterpret_cast<float2*>(hsum + r1 * LD + 8 * j + 2 * t) = make_float2(acc[j][2] + v.x, acc[j][3] + v.y);
+    }
+  }
+  const float sc = p.scale[tile.x];
+  float* fin = hsum;
+  if (c > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    const int rows = 64 / c;
+    for (int i = tid * 4; i < rows * 8 * RT; i += 1024) {
+      const int at = (rank_cta * rows + i / (8 * RT)) * LD + i % (8 * RT);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < c; ++q) {
+        const float4 w = *reinterpret_cast<const float4*>(cl.map_shared_rank(hsum, q) + at);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      for (int q = 0; q < c; ++q) *reinterpret_cast<float4*>(cl.map_shared_rank(hfin, q) + at) = v;
+    }
+    cl.sync();                                         // nobody reaches into a peer after this
+    fin = hfin;
+  } else {
+    __syncthreads();
+  }
+  if (p.h != nullptr && rank_cta == 0) {
+    for (int i = tid * 2; i < tile.z * p.r; i += 512) {
+      const int row = i / p.r, q = i % p.r;
+      uint32_t hi, lo;
+      split2(fin[row * LD + q] * sc, fin[row * LD + q + 1] * sc, hi, lo);
+      const size_t at = static_cast<size_t>(tile.y + row) * p.r + q;
+      *reinterpret_cast<uint32_t*>(p.h + at) = hi;
+      *reinterpret_cast<uint32_t*>(p.h + static_cast<size_t>(p.T) * p.r + at) = lo;
+    }
+  }
+  if (p.out == nullptr) return;
+
+  // ---- second product
+  uint32_t hi[KS][4], lo[KS][4];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int q = 16 * s + 2 * t;
+    const float2 z = make_float2(0.f, 0.f);
+    const float2 f0 = *reinterpret_cast<const float2*>(fin + r0 * LD + q), f1 = *reinterpret_cast<const float2*>(fin + r1 * LD + q);
+    const float2 f2 = RT == 1 ? z : *reinterpret_cast<const float2*>(fin + r0 * LD + q + 8), f3 = RT == 1 ? z : *reinterpret_cast<const float2*>(fin + r1 * LD + q + 8);
+    split2(f0.x * sc, f0.y * sc, hi[s][0], lo[s][0]);
+    split2(f1.x * sc, f1.y * sc, hi[s][1], lo[s][1]);
+    split2(f2.x * sc, f2.y * sc, hi[s][2], lo[s][2]);
+    split2(f3.x * sc, f3.y * sc, hi[s][3], lo[s][3]);
+  }
+  const int sa = mt * 16 + g, sb = sa + 8;             // rows that this lane stores, piece hf * 4 + t
+  __nv_bfloat16* outa = p.out + static_cast<long long>(p.perm[tile.y + (sa < tile.z ? sa : 0)]) * p.ld_out;
+  __nv_bfloat16* outb = p.out + static_cast<long long>(p.perm[tile.y + (sb < tile.z ? sb : 0)]) * p.ld_out;
+  for (int i = nk; i < total; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    __syncthreads();
+    load(i + kRing - 1);
+    const uint32_t st = ring + (i % kRing) * tile_stage<RT>(), fs = st + 8192;
+    auto factor = [&](int oct, int j) {                // address of this lane's row of the matrix (8 ranks oct) x (8 columns j)
+      if constexpr (ACROSS) return fs + wide_at(oct * 8 + l8, hf * 4 + j);
+      else return fs + narrow_at<RT>(hf * 32 + j * 8 + l8, oct);
+    };
+    auto fetch = [&](uint32_t at, uint32_t(&b)[4]) {
+      if constexpr (ACROSS) ldsm4t(at, b);
+      else ldsm4(at, b);
+    };
+    float o[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[j][q] = 0.f;
+    if constexpr (RT == 1) {
+      uint32_t b[4];
+      fetch(factor(0, lm), b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mma16816(o[j], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b[j], 0u);
+        mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[j], 0u);
+      }
+    } else if constexpr (RT == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        uint32_t b[4];
+        fetch(factor(lm & 1, j + (lm >> 1)), b);
+        mma16816(o[j], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b[0], b[1]);
+        mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[0], b[1]);
+        mma16816(o[j + 1], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b[2], b[3]);
+        mma16816(o[j + 1], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[2], b[3]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < RT / 4; ++q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b[4];
+          fetch(factor(4 * q + lm, j), b);
+          mma16816(o[j], hi[2 * q][0], hi[2 * q][1], hi[2 * q][2], hi[2 * q][3], b[0], b[1]);
+          mma16816(o[j], lo[2 * q][0], lo[2 * q][1], lo[2 * q][2], lo[2 * q][3], b[0], b[1]);
+          mma16816(o[j], hi[2 * q + 1][0], hi[2 * q + 1][1], hi[2 * q + 1][2], hi[2 * q + 1][3], b[2], b[3]);
+          mma16816(o[j], lo[2 * q + 1][0], lo[2 * q + 1][1], lo[2 * q + 1][2], lo[2 * q + 1][3], b[2], b[3]);
+        }
+      }
+    }
+    // the sum replaces the base in the stage (rows and pieces of this warp alone), so that rows leave 64 bytes at a time
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t at = st + wide_at(mt * 16 + g + 8 * u, hf * 4 + j) + t * 4;
+        float2 y = make_float2(0.f, 0.f);
+        if (p.base != nullptr) {
+          uint32_t w;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+          const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w);
+          y = make_float2(__low2float(v), __high2float(v));
+        }
+        const __nv_bfloat162 v = __floats2bfloat162_rn(y.x + o[j][2 * u], y.y + o[j][2 * u + 1]);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(*reinterpret_cast<const uint32_t*>(&v)) : "memory");
+      }
+    }
+    __syncwarp();
+    const int col = (n_lo + i - nk) * 64 + (hf * 4 + t) * 8;
+    uint4 w0, w1;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w0.x), "=r"(w0.y), "=r"(w0.z), "=r"(w0.w) : "r"(st + wide_at(sa, hf * 4 + t)) : "memory");
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w1.x), "=r"(w1.y), "=r"(w1.z), "=r"(w1.w) : "r"(st + wide_at(sb, hf * 4 + t)) : "memory");
+    if (col < p.N) {
+      if (sa < tile.z) *reinterpret_cast<uint4*>(outa + col) = w0;
+      if (sb < tile.z) *reinterpret_cast<uint4*>(outb + col) = w1;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // ------------------------------------------------------------------------------------------------ gradients of the factors
 // G[rank, col] = sum over an adapter's tokens of h[t, rank] z[t, col]. A CTA owns 128 columns of one adapter, its cluster
-// splits the adapter's tokens; a warp owns 16 columns and all ranks. Tokens are the contracted index, so both operands are
-// read across (transposed reads of shared memory) from tiles of 32 tokens that asynchronous copies bring in kStages deep.
-// h is the two bf16 numbers that lora_apply_kernel stored; sums are fp32, partial sums of the cluster are added in order.
+// splits the adapter's tokens. Tokens are the contracted index, so both operands are read across (transposed reads of
+// shared memory) from tiles of 64 tokens that asynchronous copies bring in kStages deep; a thread looks up the rows it
+// copies one tile ahead. Warp (w, f) owns 32 columns, all ranks and one half of a tile's tokens. h is the two bf16 numbers
+// that the kernels above stored; sums are fp32, those of the halves and of the cluster are added in order.
 struct GradArgs {
   const __nv_bfloat16* h;     // [2, T, r], plan's order
   const __nv_bfloat16* z;     // [T, C] rows by token
@@ -395,106 +673,128 @@ struct GradArgs {
   long long ld_z;
   int T, C, r, by_cols;
 };
-constexpr int kTok = 32, kCols = 128, kStages = 4;
+constexpr int kTok = 64, kCols = 128, kStages = 3;
 constexpr int kZRow = kCols * 2 + 16;                  // bytes a row in shared memory: 16 more spread the transposed reads
 
 template <int RT>
 constexpr int grad_stage() {
-  return kTok * kZRow + 2 * kTok * (8 * RT * 2 + 16);
+  return kTok * kZRow + 2 * kTok * 16 * RT;
 }
 template <int RT>
 constexpr int grad_smem() {
-  const int ring = kStages * grad_stage<RT>(), sums = kCols * (8 * RT + 1) * 4;
+  const int ring = kStages * grad_stage<RT>(), sums = 2 * kCols * (8 * RT + 1) * 4;
   return ring > sums ? ring : sums;
-}
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
 template <int RT>
 __global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ GradArgs p) {
-  constexpr int kHRow = 8 * RT * 2 + 16;
-  extern __shared__ __align__(16) uint8_t ring[];
+  extern __shared__ __align__(128) uint8_t raw[];
   const int c = gridDim.x, rank_cta = blockIdx.x, a = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l8 = lane & 7, lm = lane >> 3;
+  const int cg4 = warp & 3, hf = warp >> 2;
   const int col0 = blockIdx.y * kCols;
   const int t0 = p.offsets[a], t1 = p.offsets[a + 1];
   const int tiles = (t1 - t0 + kTok - 1) / kTok;
   const int lo = static_cast<int>(static_cast<long long>(tiles) * rank_cta / c), hi = static_cast<int>(static_cast<long long>(tiles) * (rank_cta + 1) / c);
-  const uint32_t base = smem_u32(ring);
-  constexpr int kHVec = RT;                            // 16-byte pieces a row of h
-  auto load = [&](int tile) {
+  const uint32_t base = smem_u32(raw);
+  // this thread copies piece ch of rows rr + 16 i
+  const int rr = tid >> 4, ch = tid & 15;
+  const bool in = col0 + ch * 8 < p.C;
+  const __nv_bfloat16* zc = p.z + (in ? col0 + ch * 8 : 0);
+  int next[4];
+  auto look = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = t0 + tile * kTok + rr + 16 * i;
+      next[i] = tile < hi && at < t1 ? p.perm[at] : -1;
+    }
+  };
+  auto load = [&](int tile) {                          // after look(tile)
     if (tile < hi) {
       const uint32_t st = base + (tile % kStages) * grad_stage<RT>();
       const int first = t0 + tile * kTok;
-      for (int i = threadIdx.x; i < kTok * (kCols / 8); i += 256) {
-        const int row = i / (kCols / 8), v = i % (kCols / 8);
-        const bool ok = first + row < t1 && col0 + v * 8 < p.C;
-        const __nv_bfloat16* src = p.z;
-        if (ok) src += static_cast<long long>(p.perm[first + row]) * p.ld_z + col0 + v * 8;
-        cp16(st + row * kZRow + v * 16, src, ok);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool ok = in && next[i] >= 0;
+        cp16(st + (rr + 16 * i) * kZRow + ch * 16, ok ? zc + static_cast<long long>(next[i]) * p.ld_z : p.z, ok);
       }
-      for (int i = threadIdx.x; i < 2 * kTok * kHVec; i += 256) {
-        const int part = i / (kTok * kHVec), row = i / kHVec % kTok, v = i % kHVec;
+#pragma unroll
+      for (int i = tid; i < 2 * kTok * RT; i += 256) {
+        const int part = i / (kTok * RT), row = i / RT % kTok, v = i % RT;
         const bool ok = first + row < t1 && v * 8 < p.r;
-        const __nv_bfloat16* src = p.h;
-        if (ok) src += (static_cast<size_t>(part) * p.T + first + row) * p.r + v * 8;
-        cp16(st + kTok * kZRow + (part * kTok + row) * kHRow + v * 16, src, ok);
+        cp16(st + kTok * kZRow + part * kTok * 16 * RT + narrow_at<RT>(row, v),
+             ok ? p.h + (static_cast<size_t>(part) * p.T + first + row) * p.r + v * 8 : p.h, ok);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  float acc[RT][4];
+  float acc[2][RT][4];
 #pragma unroll
-  for (int j = 0; j < RT; ++j)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    for (int j = 0; j < RT; ++j)
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load(lo + s);
+      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    look(lo + s);
+    load(lo + s);
+  }
+  look(lo + kStages - 1);
   for (int tile = lo; tile < hi; ++tile) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();                                   // the tile has landed, and everybody is done with the one before
     load(tile + kStages - 1);
+    look(tile + kStages);
     const uint32_t st = base + (tile % kStages) * grad_stage<RT>();
     const uint32_t hs = st + kTok * kZRow;
 #pragma unroll
-    for (int k = 0; k < kTok; k += 16) {
+    for (int s = 0; s < 2; ++s) {
+      const int k = hf * 32 + s * 16;
       // columns are the rows of the product: matrices (tokens k..k+7 | k+8..k+15) x (columns 0..7 | 8..15)
-      uint32_t za[4];
-      ldsm4t(st + (k + (lane & 7) + 8 * (lane >> 4)) * kZRow + (warp * 16 + 8 * ((lane >> 3) & 1)) * 2, za);
+      uint32_t za[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) ldsm4t(st + (k + l8 + 8 * (lm >> 1)) * kZRow + (cg4 * 32 + m * 16 + 8 * (lm & 1)) * 2, za[m]);
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
         uint32_t b[4];                                 // (hi, lo) x (tokens k..k+7 | k+8..k+15)
-        ldsm4t(hs + ((lane >> 4) * kTok + k + (lane & 7) + 8 * ((lane >> 3) & 1)) * kHRow + j * 16, b);
-        mma16816(acc[j], za[0], za[1], za[2], za[3], b[0], b[1]);
-        mma16816(acc[j], za[0], za[1], za[2], za[3], b[2], b[3]);
+        ldsm4t(hs + (lm >> 1) * kTok * 16 * RT + narrow_at<RT>(k + l8 + 8 * (lm & 1), j), b);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma16816(acc[m][j], za[m][0], za[m][1], za[m][2], za[m][3], b[0], b[1]);
+          mma16816(acc[m][j], za[m][0], za[m][1], za[m][2], za[m][3], b[2], b[3]);
+        }
       }
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  // sums of this CTA: [column][rank]
+  // sums of this CTA: [half][column][rank]
   constexpr int LD = 8 * RT + 1;
-  float* mine = reinterpret_cast<float*>(ring);
+  float* mine = reinterpret_cast<float*>(raw);
   {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      float* w = mine + (warp * 16 + g) * LD + 8 * j + 2 * t;
-      w[0] = acc[j][0], w[1] = acc[j][1];
-      w[8 * LD] = acc[j][2], w[8 * LD + 1] = acc[j][3];
-    }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        float* w = mine + (hf * kCols + cg4 * 32 + m * 16 + g) * LD + 8 * j + 2 * t;
+        w[0] = acc[m][j][0], w[1] = acc[m][j][1];
+        w[8 * LD] = acc[m][j][2], w[8 * LD + 1] = acc[m][j][3];
+      }
   }
   cg::cluster_group cl = cg::this_cluster();
   cl.sync();
   const int cols = min(kCols, p.C - col0);
   __nv_bfloat16* out = p.out + static_cast<size_t>(a) * p.r * p.C;
   // the cluster's CTAs share the output's elements
-  for (int i = rank_cta * 256 + threadIdx.x; i < cols * p.r; i += c * 256) {
+  for (int i = rank_cta * 256 + tid; i < cols * p.r; i += c * 256) {
     const int col = p.by_cols ? i / p.r : i % cols, q = p.by_cols ? i % p.r : i / cols;
     float v = 0.f;
-    for (int k = 0; k < c; ++k) v += cl.map_shared_rank(mine, k)[col * LD + q];
+    for (int k = 0; k < c; ++k) {
+      const float* w = cl.map_shared_rank(mine, k) + col * LD + q;
+      v += w[0] + w[kCols * LD];
+    }
     out[p.by_cols ? static_cast<size_t>(col0 + col) * p.r + q : static_cast<size_t>(q) * p.C + col0 + col] = __float2bfloat16_rn(v);
   }
   cl.sync();
@@ -518,14 +818,12 @@ int launch_cluster(void (*kern)(Args), const Args& args, dim3 grid, int cluster,
   return 0;
 }
 
-template <int RT, int MT>
-int apply_across(const ApplyArgs& a, int across, dim3 grid, cudaStream_t s) {
-  if (across) return launch_cluster(lora_apply_kernel<RT, MT, true>, a, grid, grid.x, apply_smem<RT, MT>(true), s);
-  return launch_cluster(lora_apply_kernel<RT, MT, false>, a, grid, grid.x, apply_smem<RT, MT>(false), s);
-}
 template <int RT>
 int apply_tile(const ApplyArgs& a, int large, int across, dim3 grid, cudaStream_t s) {
-  return large ? apply_across<RT, kLarge / 16>(a, across, grid, s) : apply_across<RT, 1>(a, across, grid, s);
+  if (large && across) return launch_cluster(lora_tile_kernel<RT, true>, a, grid, grid.x, tile_smem<RT>(), s);
+  if (large) return launch_cluster(lora_tile_kernel<RT, false>, a, grid, grid.x, tile_smem<RT>(), s);
+  if (across) return launch_cluster(lora_apply_kernel<RT, true>, a, grid, grid.x, apply_smem<RT>(true), s);
+  return launch_cluster(lora_apply_kernel<RT, false>, a, grid, grid.x, apply_smem<RT>(false), s);
 }
 
 inline int bound_tiles(int T, int E, int size) {
@@ -583,7 +881,7 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   // CTAs a tile: until the card has three a multiprocessor, but not beyond one step of 32 a warp
   int c = 1;
   const int widest = (K > N ? K : N) / 32;
-  while (c < 8 && tiles * c < 148 * 3 && widest > c * (large ? 2 : 8)) c *= 2;
+  while (c < 8 && tiles * c < 148 * 3 && widest > c * 8) c *= 2;
   const dim3 grid(c, tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (r <= 8) return apply_tile<1>(a, large, across, grid, s);
