@@ -104,7 +104,7 @@ lora_plan_kernel(const int* __restrict__ ids, int T, int E, int* __restrict__ pe
 
 // ------------------------------------------------------------------------------------------------ fragments
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -112,8 +112,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ uint4 ld16(const __nv_bfloat16* p, bool ok) {
   return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
@@ -257,10 +256,13 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
     for (int i = threadIdx.x * 4; i < kVals; i += kWarps * 32 * 4) {
       const int at = (i / (8 * RT)) * LD + i % (8 * RT);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < c; ++q) {
-        const float4 w = *reinterpret_cast<const float4*>(cl.map_shared_rank(sum, q) + at);
-        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-      }
+      float4 w[8];                                     // all of them asked for before the first is used
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < c) w[q] = *reinterpret_cast<const float4*>(cl.map_shared_rank(sum, q) + at);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < c) v.x += w[q].x, v.y += w[q].y, v.z += w[q].z, v.w += w[q].w;
       *reinterpret_cast<float4*>(fin + at) = make_float4(v.x * sc, v.y * sc, v.z * sc, v.w * sc);
     }
     cl.sync();                                         // nobody reads a peer's sum after this
@@ -384,7 +386,9 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
 // for, this one keeps in flight: a ring of kRing stages that asynchronous copies fill, 64 of K (or of N) by the tile's 64
 // rows and the factor's part, goes on through both products, so the columns' first stages are under way while the cluster
 // adds up h. Warp (m, f) owns 16 rows and one half of a stage. A stage is stored in 16-byte pieces whose place within the
-// row is xored with the row's number: reads of 8 rows at once meet 8 different bank groups.
+// row is xored with bits of the row's number: reads of 8 rows at once, and of 2 rows' half lines, meet 8 different bank
+// groups. The loop was bound by its instructions at first (69 % of issue slots, 4.8 TB/s), so what a thread copies next is
+// held as running pointers.
 constexpr int kRing = 4;
 
 template <int RT>
@@ -401,19 +405,52 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 // byte of a 16-byte piece: rows of 8 pieces (64 numbers), or of RT pieces (the rank)
-__device__ __forceinline__ uint32_t wide_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint32_t wide_at(int row, int piece) { return row * 128 + ((piece ^ (((row & 1) << 2) | ((row >> 1) & 3))) << 4); }
 template <int RT>
 __device__ __forceinline__ uint32_t narrow_at(int row, int piece) {
   const int x = RT >= 8 ? row & 7 : RT == 4 ? (row >> 1) & 3 : RT == 2 ? (row >> 2) & 1 : 0;
   return row * 16 * RT + ((piece ^ x) << 4);
 }
 
+// What one thread copies of a factor's part of a stage: piece v of rows row, row + kRows, ... The rows are ranks (8 RT of
+// them, 64 numbers wide) or places along K / N (64 of them, the rank wide); SPREAD stores those places so that the 8 rows
+// of a matrix are columns a lane then holds side by side (see the second product).
+template <int RT, bool RANKS, bool SPREAD>
+struct Feed {
+  static constexpr int kTimes = (64 * RT + 255) / 256, kRows = RANKS ? 32 : 256 / RT;
+  const __nv_bfloat16* src;
+  int at, width, r;                     // first number (RANKS), or place, of this thread's next piece
+  bool ok;
+  __device__ __forceinline__ Feed(const __nv_bfloat16* f, int start, int width_, int r_) : width(width_), r(r_) {
+    const int row = RANKS ? threadIdx.x >> 3 : threadIdx.x / RT, v = RANKS ? threadIdx.x & 7 : threadIdx.x % RT;
+    ok = RANKS || v * 8 < r;
+    at = start + (RANKS ? v * 8 : row);
+    src = f + (RANKS ? static_cast<size_t>(row) * width + at : static_cast<size_t>(at) * r + v * 8);
+  }
+  __device__ __forceinline__ void copy(uint32_t dst, const __nv_bfloat16* anywhere) {
+    const int row0 = RANKS ? threadIdx.x >> 3 : threadIdx.x / RT, v = RANKS ? threadIdx.x & 7 : threadIdx.x % RT;
+    if (RT >= 4 || threadIdx.x < 64 * RT) {
+#pragma unroll
+      for (int i = 0; i < kTimes; ++i) {
+        int row = row0 + i * kRows;
+        const bool in = RANKS ? at < width && (RT <= 2 || row < r) : ok && at + i * kRows < width;
+        const __nv_bfloat16* from = src + (RANKS ? static_cast<size_t>(i * kRows) * width : static_cast<size_t>(i * kRows) * r);
+        if (SPREAD) row = (row & 32) | (((row >> 1) & 3) << 3) | (((row >> 3) & 3) << 1) | (row & 1);
+        cp16(dst + (RANKS ? wide_at(row, v) : narrow_at<RT>(row, v)), in ? from : anywhere, in);
+      }
+    }
+    at += 64;
+    src += RANKS ? 64 : 64 * r;
+  }
+};
+
+// CTAs a multiprocessor are what keeps its memory busy: the compiler is held to the registers that allow 4 (rank 16: 212 us
+// at 8192 x 4096 -> 24576 with 3, 187 with 4) or 3 and 2 for the larger ranks (64: 87 us with 1 at 4096 -> 4096, 66 with 2)
 template <int RT, bool ACROSS>
-__global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ ApplyArgs p) {
+__global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT <= 4 ? 3 : RT <= 8 ? 2 : 1) lora_tile_kernel(const __grid_constant__ ApplyArgs p) {
   constexpr int LD = 8 * RT + 4;
   constexpr int KS = RT < 2 ? 1 : RT / 2;
   extern __shared__ __align__(128) uint8_t raw[];
@@ -445,47 +482,33 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
   const int nk = k_hi - k_lo, total = nk + (p.out != nullptr ? n_hi - n_lo : 0);
   const __nv_bfloat16* down = p.down + static_cast<size_t>(tile.x) * p.r * p.K;
   const __nv_bfloat16* up = p.up + static_cast<size_t>(tile.x) * p.r * p.N;
-  auto wide = [&](uint32_t dst, const __nv_bfloat16* f, int width, int at) {     // rows: ranks
-#pragma unroll
-    for (int i = tid; i < 64 * RT; i += 256) {
-      const int row = i >> 3, v = i & 7;
-      const bool ok = row < p.r && at + v * 8 < width;
-      cp16(dst + wide_at(row, v), ok ? f + static_cast<size_t>(row) * width + at + v * 8 : f, ok);
-    }
-  };
-  auto narrow = [&](uint32_t dst, const __nv_bfloat16* f, int width, int at) {   // rows: K or N
-#pragma unroll
-    for (int i = tid; i < 64 * RT; i += 256) {
-      const int row = i / RT, v = i % RT;
-      const bool ok = at + row < width && v * 8 < p.r;
-      cp16(dst + narrow_at<RT>(row, v), ok ? f + static_cast<size_t>(at + row) * p.r + v * 8 : f, ok);
-    }
-  };
-  auto load = [&](int i) {
-    if (i < total) {
-      const uint32_t st = ring + (i % kRing) * tile_stage<RT>();
-      if (i < nk) {
-        const int k = (k_lo + i) * 64;
-        const bool in = k + ch * 8 < p.K;
-        cp16(st + wide_at(ra, ch), in ? p.in + rowa * p.ld_in + k + ch * 8 : p.in, in && oka);
-        cp16(st + wide_at(rb, ch), in ? p.in + rowb * p.ld_in + k + ch * 8 : p.in, in && okb);
-        if constexpr (ACROSS) narrow(st + 8192, down, p.K, k);
-        else wide(st + 8192, down, p.K, k);
-      } else {
-        const int n = (n_lo + i - nk) * 64;
-        const bool in = n + ch * 8 < p.N;
-        if (p.base != nullptr) {
-          cp16(st + wide_at(ra, ch), in ? p.base + rowa * p.ld_base + n + ch * 8 : p.base, in && oka);
-          cp16(st + wide_at(rb, ch), in ? p.base + rowb * p.ld_base + n + ch * 8 : p.base, in && okb);
-        }
-        if constexpr (ACROSS) wide(st + 8192, up, p.N, n);
-        else narrow(st + 8192, up, p.N, n);
+  Feed<RT, !ACROSS, false> feed_down(down, k_lo * 64, p.K, p.r);
+  Feed<RT, ACROSS, !ACROSS> feed_up(up, n_lo * 64, p.N, p.r);
+  const uint32_t da = wide_at(ra, ch), db = wide_at(rb, ch);
+  const __nv_bfloat16 *pa = p.in + rowa * p.ld_in + k_lo * 64 + ch * 8, *pb = p.in + rowb * p.ld_in + k_lo * 64 + ch * 8;
+  int col = k_lo * 64 + ch * 8, fed = 0;
+  uint32_t slot = ring;                                // where the next stage goes
+  auto load = [&]() {
+    if (fed < total) {
+      if (fed == nk) {
+        pa = p.base + rowa * p.ld_base + n_lo * 64 + ch * 8, pb = p.base + rowb * p.ld_base + n_lo * 64 + ch * 8;
+        col = n_lo * 64 + ch * 8;
       }
+      const bool first = fed < nk, in = col < (first ? p.K : p.N);
+      if (first || p.base != nullptr) {
+        cp16(slot + da, in ? pa : p.in, in && oka);
+        cp16(slot + db, in ? pb : p.in, in && okb);
+      }
+      if (first) feed_down.copy(slot + 8192, p.in);
+      else feed_up.copy(slot + 8192, p.in);
+      pa += 64, pb += 64, col += 64;
+      ++fed;
+      slot = slot == ring + (kRing - 1) * tile_stage<RT>() ? ring : slot + tile_stage<RT>();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) load(i);
+  for (int i = 0; i < kRing - 1; ++i) load();
 
   // ---- first product
   float acc[RT][4];
@@ -494,11 +517,12 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
   const int l8 = lane & 7, lm = lane >> 3;             // row and matrix that this lane's address is for
+  uint32_t st = ring;                                  // the stage that is read
   for (int i = 0; i < nk; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
     __syncthreads();                                   // the stage has landed, and everybody is done with the one before
-    load(i + kRing - 1);
-    const uint32_t st = ring + (i % kRing) * tile_stage<RT>(), fs = st + 8192;
+    load();
+    const uint32_t fs = st + 8192;
     uint32_t a[2][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) ldsm4(st + wide_at(mt * 16 + l8 + 8 * (lm & 1), hf * 4 + 2 * s + (lm >> 1)), a[s]);
@@ -510,6 +534,7 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
       mma16816(acc[j], a[0][0], a[0][1], a[0][2], a[0][3], b[0], b[1]);
       mma16816(acc[j], a[1][0], a[1][1], a[1][2], a[1][3], b[2], b[3]);
     }
+    st = st == ring + (kRing - 1) * tile_stage<RT>() ? ring : st + tile_stage<RT>();
   }
 
   // ---- h: the two halves, then the cluster in order: each CTA adds up its share of the rows and hands it to all
@@ -539,11 +564,16 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
     for (int i = tid * 4; i < rows * 8 * RT; i += 1024) {
       const int at = (rank_cta * rows + i / (8 * RT)) * LD + i % (8 * RT);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < c; ++q) {
-        const float4 w = *reinterpret_cast<const float4*>(cl.map_shared_rank(hsum, q) + at);
-        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-      }
-      for (int q = 0; q < c; ++q) *reinterpret_cast<float4*>(cl.map_shared_rank(hfin, q) + at) = v;
+      float4 w[8];                                     // all of them asked for before the first is used
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < c) w[q] = *reinterpret_cast<const float4*>(cl.map_shared_rank(hsum, q) + at);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < c) v.x += w[q].x, v.y += w[q].y, v.z += w[q].z, v.w += w[q].w;
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < c) *reinterpret_cast<float4*>(cl.map_shared_rank(hfin, q) + at) = v;
     }
     cl.sync();                                         // nobody reaches into a peer after this
     fin = hfin;
@@ -578,11 +608,12 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
   const int sa = mt * 16 + g, sb = sa + 8;             // rows that this lane stores, piece hf * 4 + t
   __nv_bfloat16* outa = p.out + static_cast<long long>(p.perm[tile.y + (sa < tile.z ? sa : 0)]) * p.ld_out;
   __nv_bfloat16* outb = p.out + static_cast<long long>(p.perm[tile.y + (sb < tile.z ? sb : 0)]) * p.ld_out;
-  for (int i = nk; i < total; ++i) {
+  int oc = n_lo * 64 + (hf * 4 + t) * 8;               // first of the 8 columns that this lane stores
+  for (int i = nk; i < total; ++i, oc += 64) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
     __syncthreads();
-    load(i + kRing - 1);
-    const uint32_t st = ring + (i % kRing) * tile_stage<RT>(), fs = st + 8192;
+    load();
+    const uint32_t fs = st + 8192;
     auto factor = [&](int oct, int j) {                // address of this lane's row of the matrix (8 ranks oct) x (8 columns j)
       if constexpr (ACROSS) return fs + wide_at(oct * 8 + l8, hf * 4 + j);
       else return fs + narrow_at<RT>(hf * 32 + j * 8 + l8, oct);
@@ -628,32 +659,51 @@ __global__ void __launch_bounds__(256) lora_tile_kernel(const __grid_constant__ 
         }
       }
     }
-    // the sum replaces the base in the stage (rows and pieces of this warp alone), so that rows leave 64 bytes at a time
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t at = st + wide_at(mt * 16 + g + 8 * u, hf * 4 + j) + t * 4;
-        float2 y = make_float2(0.f, 0.f);
-        if (p.base != nullptr) {
-          uint32_t w;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-          const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w);
-          y = make_float2(__low2float(v), __high2float(v));
-        }
-        const __nv_bfloat162 v = __floats2bfloat162_rn(y.x + o[j][2 * u], y.y + o[j][2 * u + 1]);
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(*reinterpret_cast<const uint32_t*>(&v)) : "memory");
-      }
-    }
-    __syncwarp();
-    const int col = (n_lo + i - nk) * 64 + (hf * 4 + t) * 8;
     uint4 w0, w1;
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w0.x), "=r"(w0.y), "=r"(w0.z), "=r"(w0.w) : "r"(st + wide_at(sa, hf * 4 + t)) : "memory");
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w1.x), "=r"(w1.y), "=r"(w1.z), "=r"(w1.w) : "r"(st + wide_at(sb, hf * 4 + t)) : "memory");
-    if (col < p.N) {
-      if (sa < tile.z) *reinterpret_cast<uint4*>(outa + col) = w0;
-      if (sb < tile.z) *reinterpret_cast<uint4*>(outb + col) = w1;
+    if constexpr (!ACROSS) {
+      // tile j holds the columns 8 t + 2 j of this half: the lane has 8 neighbours of each of its rows
+      uint4 y0 = make_uint4(0u, 0u, 0u, 0u), y1 = y0;
+      if (p.base != nullptr) {
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(y0.x), "=r"(y0.y), "=r"(y0.z), "=r"(y0.w) : "r"(st + wide_at(sa, hf * 4 + t)) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(y1.x), "=r"(y1.y), "=r"(y1.z), "=r"(y1.w) : "r"(st + wide_at(sb, hf * 4 + t)) : "memory");
+      }
+      const __nv_bfloat162* b0 = reinterpret_cast<const __nv_bfloat162*>(&y0);
+      const __nv_bfloat162* b1 = reinterpret_cast<const __nv_bfloat162*>(&y1);
+      __nv_bfloat162* v0 = reinterpret_cast<__nv_bfloat162*>(&w0);
+      __nv_bfloat162* v1 = reinterpret_cast<__nv_bfloat162*>(&w1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v0[j] = __floats2bfloat162_rn(__low2float(b0[j]) + o[j][0], __high2float(b0[j]) + o[j][1]);
+        v1[j] = __floats2bfloat162_rn(__low2float(b1[j]) + o[j][2], __high2float(b1[j]) + o[j][3]);
+      }
+    } else {
+      // tile j holds columns 8 j of this half: the sum replaces the base in the stage (rows and pieces of this warp alone),
+      // so that rows leave 64 bytes at a time
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t at = st + wide_at(mt * 16 + g, hf * 4 + j) + u * 1024 + t * 4;
+          float2 y = make_float2(0.f, 0.f);
+          if (p.base != nullptr) {
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+            const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w);
+            y = make_float2(__low2float(v), __high2float(v));
+          }
+          const __nv_bfloat162 v = __floats2bfloat162_rn(y.x + o[j][2 * u], y.y + o[j][2 * u + 1]);
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(*reinterpret_cast<const uint32_t*>(&v)) : "memory");
+        }
+      }
+      __syncwarp();
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w0.x), "=r"(w0.y), "=r"(w0.z), "=r"(w0.w) : "r"(st + wide_at(sa, hf * 4 + t)) : "memory");
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w1.x), "=r"(w1.y), "=r"(w1.z), "=r"(w1.w) : "r"(st + wide_at(sb, hf * 4 + t)) : "memory");
     }
+    if (oc < p.N) {
+      if (sa < tile.z) *reinterpret_cast<uint4*>(outa + oc) = w0;
+      if (sb < tile.z) *reinterpret_cast<uint4*>(outb + oc) = w1;
+    }
+    st = st == ring + (kRing - 1) * tile_stage<RT>() ? ring : st + tile_stage<RT>();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -682,7 +732,7 @@ constexpr int grad_stage() {
 }
 template <int RT>
 constexpr int grad_smem() {
-  const int ring = kStages * grad_stage<RT>(), sums = 2 * kCols * (8 * RT + 1) * 4;
+  const int ring = kStages * grad_stage<RT>(), sums = kCols * (8 * RT + 4) * 4;
   return ring > sums ? ring : sums;
 }
 
@@ -769,33 +819,52 @@ __global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ 
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  // sums of this CTA: [half][column][rank]
-  constexpr int LD = 8 * RT + 1;
+  // sums of this CTA: [column][rank], the halves in order
+  constexpr int LD = 8 * RT + 4;
   float* mine = reinterpret_cast<float*>(raw);
-  {
-    const int g = lane >> 2, t = lane & 3;
+  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+  for (int turn = 1; turn >= 0; --turn) {
+    if (hf == turn) {
 #pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        float* w = mine + (hf * kCols + cg4 * 32 + m * 16 + g) * LD + 8 * j + 2 * t;
-        w[0] = acc[m][j][0], w[1] = acc[m][j][1];
-        w[8 * LD] = acc[m][j][2], w[8 * LD + 1] = acc[m][j][3];
-      }
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float2* w = reinterpret_cast<float2*>(mine + (cg4 * 32 + m * 16 + g + 8 * u) * LD + 8 * j + 2 * t);
+            float2 v = make_float2(acc[m][j][2 * u], acc[m][j][2 * u + 1]);
+            if (turn == 0) v.x += w->x, v.y += w->y;
+            *w = v;
+          }
+    }
+    if (turn == 1) __syncthreads();
   }
+  // the cluster's CTAs share the columns
   cg::cluster_group cl = cg::this_cluster();
   cl.sync();
-  const int cols = min(kCols, p.C - col0);
   __nv_bfloat16* out = p.out + static_cast<size_t>(a) * p.r * p.C;
-  // the cluster's CTAs share the output's elements
-  for (int i = rank_cta * 256 + tid; i < cols * p.r; i += c * 256) {
-    const int col = p.by_cols ? i / p.r : i % cols, q = p.by_cols ? i % p.r : i / cols;
-    float v = 0.f;
-    for (int k = 0; k < c; ++k) {
-      const float* w = cl.map_shared_rank(mine, k) + col * LD + q;
-      v += w[0] + w[kCols * LD];
+  const int share = kCols / c;
+  for (int i = tid; i < share * 2 * RT; i += 256) {
+    const int col = rank_cta * share + (p.by_cols ? i / (2 * RT) : i % share), q = 4 * (p.by_cols ? i % (2 * RT) : i / share);
+    float4 w[8], v = make_float4(0.f, 0.f, 0.f, 0.f);  // all of them asked for before the first is used
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < c) w[k] = *reinterpret_cast<const float4*>(cl.map_shared_rank(mine, k) + col * LD + q);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < c) v.x += w[k].x, v.y += w[k].y, v.z += w[k].z, v.w += w[k].w;
+    if (col0 + col < p.C && q < p.r) {
+      const __nv_bfloat162 lo2 = __floats2bfloat162_rn(v.x, v.y), hi2 = __floats2bfloat162_rn(v.z, v.w);
+      if (p.by_cols) {
+        uint2 both;
+        both.x = *reinterpret_cast<const uint32_t*>(&lo2), both.y = *reinterpret_cast<const uint32_t*>(&hi2);
+        *reinterpret_cast<uint2*>(out + static_cast<size_t>(col0 + col) * p.r + q) = both;
+      } else {
+        __nv_bfloat16* to = out + static_cast<size_t>(q) * p.C + col0 + col;
+        to[0] = lo2.x, to[p.C] = lo2.y, to[2 * static_cast<size_t>(p.C)] = hi2.x, to[3 * static_cast<size_t>(p.C)] = hi2.y;
+      }
     }
-    out[p.by_cols ? static_cast<size_t>(col0 + col) * p.r + q : static_cast<size_t>(q) * p.C + col0 + col] = __float2bfloat16_rn(v);
   }
   cl.sync();
 }
@@ -878,10 +947,13 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   a.n_tiles = static_cast<const int*>(n_tiles) + large;
   const int tiles = bound_tiles(T, E, large ? kLarge : kSmall);
   if (tiles > 65535) return ixh::fail(ixh::IX_ESIZE, "lora: %d tokens of %d adapters make more than 65535 tiles", T, E);
-  // CTAs a tile: until the card has three a multiprocessor, but not beyond one step of 32 a warp
+  // CTAs a tile: until the card has three a multiprocessor, but not beyond eight steps (small: one a warp) each; where a CTA
+  // then still has 96 stages, once more: the last CTAs to run are shorter (8192 x 4096 -> 24576: 189 us with 4, 163 with 8;
+  // 4096 -> 4096, with 32 stages: 44 us either way, but rank 64 loses from 66 to 77)
   int c = 1;
   const int widest = (K > N ? K : N) / 32;
   while (c < 8 && tiles * c < 148 * 3 && widest > c * 8) c *= 2;
+  if (large && c < 8 && (K + N) / 64 >= 96 * c) c *= 2;
   const dim3 grid(c, tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (r <= 8) return apply_tile<1>(a, large, across, grid, s);
@@ -909,9 +981,10 @@ IX_API int ix_lora_grad(const void* h, const void* z, long long ld_z, void* out,
     IX_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(E) * r * C * 2, reinterpret_cast<cudaStream_t>(stream)));
     return 0;
   }
-  // CTAs an adapter's columns: until the card has three a multiprocessor, but not beyond four tiles of tokens each
+  // CTAs an adapter's columns: until the card has two a multiprocessor, but not beyond four tiles of an average adapter's
+  // tokens each (8192 tokens x 24576: 79 us with 2, 117 with 1, 84 with 4; 463 tokens an adapter: 8 us with 2, 11 with 4)
   int c = 1;
-  while (c < 8 && tiles * E * c < 148 * 3 && T > c * 4 * kTok) c *= 2;
+  while (c < 8 && tiles * E * c < 148 * 2 && T / E > c * 4 * kTok) c *= 2;
   const dim3 grid(c, tiles, E);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (r <= 8) return launch_cluster(lora_grad_kernel<1>, a, grid, c, grad_smem<1>(), s);

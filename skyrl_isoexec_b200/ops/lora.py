@@ -9,6 +9,8 @@ different ranks share a bank when the smaller ones are filled up with zero rows 
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
 from . import _native
@@ -41,10 +43,12 @@ class LoraPlan:
         buf = torch.empty(4 * small + 4 * large + self.T + self.E + 2 + 2, dtype=torch.int32, device=ids.device)
         self.tiles_small, self.tiles_large, self.perm, self.offsets, self.n_tiles = buf.split(
             [4 * small, 4 * large, self.T, self.E + 2, 2])
+        # the addresses of the plan's own buffers: taken once, every call passes them
+        self._apply_args = (self.perm.data_ptr(), self.tiles_small.data_ptr(), self.tiles_large.data_ptr(), self.n_tiles.data_ptr())
+        self._offsets_ptr = self.offsets.data_ptr()
         with torch.cuda.device(ids.device):
-            _native.check(L.ix_lora_plan(ids.data_ptr(), self.T, self.E, self.perm.data_ptr(), self.offsets.data_ptr(),
-                                         self.tiles_small.data_ptr(), self.tiles_large.data_ptr(), self.n_tiles.data_ptr(), _native.stream()),
-                          "ix_lora_plan")
+            _native.check(L.ix_lora_plan(ids.data_ptr(), self.T, self.E, self._apply_args[0], self._offsets_ptr, *self._apply_args[1:],
+                                         _native.stream()), "ix_lora_plan")
 
 
 def pad_rank(A: torch.Tensor, B: torch.Tensor, rank: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -56,34 +60,37 @@ def pad_rank(A: torch.Tensor, B: torch.Tensor, rank: int) -> tuple[torch.Tensor,
 
 
 def _check(y, x, A, B, scale, plan) -> None:
-    if A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
-        raise ValueError(f"lora: factors are A [E, r, K] and B [E, N, r], not {tuple(A.shape)} and {tuple(B.shape)}")
-    E, r, K = A.shape
-    N = B.shape[1]
-    if x.shape[-1] != K or (y is not None and (y.shape[-1] != N or y.shape[:-1] != x.shape[:-1])):
-        raise ValueError(f"lora: x {tuple(x.shape)} and y {None if y is None else tuple(y.shape)} do not fit factors of widths {K} and {N}")
-    if plan.E != E or plan.T != x.numel() // K:
+    sa, sb, sx = A.shape, B.shape, x.shape
+    if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2]:
+        raise ValueError(f"lora: factors are A [E, r, K] and B [E, N, r], not {tuple(sa)} and {tuple(sb)}")
+    E, r, K = sa
+    N = sb[1]
+    if sx[-1] != K or (y is not None and (y.shape[-1] != N or y.shape[:-1] != sx[:-1])):
+        raise ValueError(f"lora: x {tuple(sx)} and y {None if y is None else tuple(y.shape)} do not fit factors of widths {K} and {N}")
+    if plan.E != E or plan.T * K != x.numel():
         raise ValueError(f"lora: the plan is for {plan.T} tokens of {plan.E} adapters, x has {x.numel() // K} and the bank {E}")
-    if scale.shape != (E,) or scale.dtype != torch.float32:
+    if scale.dtype != torch.float32 or scale.shape != (E,):
         raise ValueError(f"lora: scale is fp32 [{E}], not {tuple(scale.shape)} {scale.dtype}")
     if scale.requires_grad:
         raise ValueError("lora: scale is a constant, it has no gradient")
-    ts = [t for t in (y, x, A, B) if t is not None]
-    if any(t.device != plan.device for t in ts) or scale.device != plan.device:
+    dev, dt = plan.device, x.dtype
+    if x.device != dev or A.device != dev or B.device != dev or scale.device != dev or (y is not None and y.device != dev):
         raise ValueError("lora: all tensors and the plan are on one device")
-    if any(t.dtype != x.dtype for t in ts):
+    if A.dtype != dt or B.dtype != dt or (y is not None and y.dtype != dt):
         raise ValueError("lora: x, y, A and B have one type")
     if x.is_cuda:
-        if x.dtype != torch.bfloat16:
-            raise ValueError(f"lora: on a GPU the tensors are bf16, not {x.dtype}")
+        if dt != torch.bfloat16:
+            raise ValueError(f"lora: on a GPU the tensors are bf16, not {dt}")
         if r % 8 or r > MAX_RANK or K % 8 or N % 8:
             raise ValueError(f"lora: rank {r} (a multiple of 8 up to {MAX_RANK}: pad_rank) and widths {K}, {N} (multiples of 8)")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[T, width] with unit inner stride, rows on 16-byte boundaries."""
-    t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] and (t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16):
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    st = t.stride()
+    if (st[1] != 1 or st[0] % 8 or t.data_ptr() % 16) and t.shape[0]:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
@@ -91,8 +98,14 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _factor(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
+
+
+def _device_of(x: torch.Tensor):
+    """Makes x's device current; nothing where it is (the usual case, and microseconds of a small call)."""
+    return nullcontext() if torch.cuda.current_device() == x.get_device() else torch.cuda.device(x.device)
 
 
 def _apply(x, base, out, down, up, scale, plan, across, want_h):
@@ -106,8 +119,7 @@ def _apply(x, base, out, down, up, scale, plan, across, want_h):
     _native.check(
         _native.lib().ix_lora_apply(x.data_ptr(), x.stride(0), _native.ptr(base), base.stride(0) if base is not None else 0, _native.ptr(out),
                                     out.stride(0) if out is not None else 0, down.data_ptr(), up.data_ptr(), scale.data_ptr(),
-                                    plan.perm.data_ptr(), plan.tiles_small.data_ptr(), plan.tiles_large.data_ptr(), plan.n_tiles.data_ptr(),
-                                    _native.ptr(h), T, K, N, r, E, int(across), _native.stream()),
+                                    *plan._apply_args, _native.ptr(h), T, K, N, r, E, int(across), _native.raw_stream(x.get_device())),
         "ix_lora_apply")
     return h
 
@@ -116,8 +128,8 @@ def _factor_grad(h, z, like, plan, by_cols):
     out = torch.empty_like(like, memory_format=torch.contiguous_format)
     r, C = (like.shape[2], like.shape[1]) if by_cols else (like.shape[1], like.shape[2])
     _native.check(
-        _native.lib().ix_lora_grad(h.data_ptr(), z.data_ptr(), z.stride(0), out.data_ptr(), plan.perm.data_ptr(), plan.offsets.data_ptr(),
-                                   plan.T, C, r, plan.E, int(by_cols), _native.stream()),
+        _native.lib().ix_lora_grad(h.data_ptr(), z.data_ptr(), z.stride(0), out.data_ptr(), plan._apply_args[0], plan._offsets_ptr,
+                                   plan.T, C, r, plan.E, int(by_cols), _native.raw_stream(z.get_device())),
         "ix_lora_grad")
     return out
 
@@ -146,7 +158,7 @@ def _cpu_grad(h, z, plan):
 def _forward(y, x, A, B, scale, plan, inplace: bool, want_h: bool):
     """(out, h) on rows; ``inplace``: out is y."""
     if x.is_cuda:
-        with torch.cuda.device(x.device):
+        with _device_of(x):
             out = y if inplace else torch.empty(y.shape, dtype=y.dtype, device=y.device)
             return out, _apply(x, y, out, A, B, scale, plan, False, want_h)
     h = _cpu_h(x, A, scale, plan)
@@ -159,7 +171,7 @@ def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, nee
     """(dx, dA, dB); ``base``: the other part of dx, added to in place."""
     dx = dA = dB = None
     if x.is_cuda:
-        with torch.cuda.device(x.device):
+        with _device_of(x):
             g = None
             if need_x or need_a:
                 dx = None if not need_x else base if base is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -223,9 +235,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     """``y + s_a (x A_a^T) B_a^T`` for every token's own adapter: x [..., K], y [..., N], A [E, r, K], B [E, N, r], scale [E].
     One rounding, of the result; a token without an adapter gets y's bits. Differentiable in y, x, A and B."""
     _check(y, x, A, B, scale, plan)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, A, B)):
+    if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or y.requires_grad):
         return _LoraAdd.apply(y, x, A, B, scale, plan)
-    return _forward(_rows(y), _rows(x), _factor(A), _factor(B), scale, plan, False, False)[0].view(y.shape)
+    out = _forward(_rows(y), _rows(x), _factor(A), _factor(B), scale, plan, False, False)[0]
+    return out if y.dim() == 2 else out.view(y.shape)
 
 
 def lora_linear(x: torch.Tensor, w: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scale: torch.Tensor, plan: LoraPlan) -> torch.Tensor:
@@ -234,7 +247,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, A: torch.Tensor, B: torch.Tens
     _check(None, x, A, B, scale, plan)
     if w.dim() != 2 or w.shape != (B.shape[1], A.shape[2]) or w.dtype != x.dtype or w.device != x.device:
         raise ValueError(f"lora: w {tuple(w.shape)} {w.dtype} does not fit factors of widths {A.shape[2]} and {B.shape[1]}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w, A, B)):
+    if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or w.requires_grad):
         return _LoraLinear.apply(x, w, A, B, scale, plan)
     x2 = _rows(x)
     return _forward(F.gemm_nt(x2, w), x2, _factor(A), _factor(B), scale, plan, True, False)[0].view(*x.shape[:-1], w.shape[0])

@@ -51,7 +51,7 @@ class TensorAdamW:
         decay = [float(weight_decay)] * len(params) if not hasattr(weight_decay, "__len__") else [float(w) for w in weight_decay]
         if len(decay) != len(params):
             raise ValueError(f"TensorAdamW: {len(decay)} weight decays for {len(params)} parameters")
-        dev, dt = params[0].device, params[0].dtype
+        dev, dt = params[0].device, params[0].dtype          # (a tensor's device always carries its index)
         if dt not in (torch.float32, torch.bfloat16):
             raise ValueError(f"TensorAdamW: parameters are fp32 or bf16, not {dt}")
         self.device, self.lr, self.betas, self.eps, self.weight_decay, self.state_bits = dev, lr, tuple(betas), eps, decay, state_bits
@@ -91,14 +91,20 @@ class TensorAdamW:
 
     def _tables(self) -> None:
         chunk = _native.lib().ix_tensor_adamw_chunk()
-        rows, pairs = bytearray(), []
-        for i, (p, g, off, wd) in enumerate(zip(self.params, self.grads, self.offsets, self.weight_decay)):
+        rows = bytearray()
+        for p, g, off, wd in zip(self.params, self.grads, self.offsets, self.weight_decay):
             vec = int(p.data_ptr() % 16 == 0 and g.data_ptr() % 16 == 0)
             rows += struct.pack("<QQqqfi24x", p.data_ptr(), g.data_ptr(), p.numel(), off, wd, vec)
-            pairs += [(i, c) for c in range(-(-p.numel() // chunk))]
-        self._n_chunks = len(pairs)
+        n = torch.tensor([-(-p.numel() // chunk) for p in self.params])
+        tensor = torch.repeat_interleave(torch.arange(len(self.params)), n)
+        piece = torch.arange(len(tensor)) - (n.cumsum(0) - n)[tensor]
         self._table = torch.frombuffer(rows, dtype=torch.uint8).to(self.device)
-        self._chunks = torch.tensor(pairs, dtype=torch.int32).reshape(-1, 2).to(self.device)
+        self._chunks = torch.stack([tensor, piece], 1).to(torch.int32).to(self.device)
+        st = self.state
+        # everything a step passes that does not change: the buffers are this object's own
+        self._args = (self._table.data_ptr(), self._chunks.data_ptr(), len(tensor), int(self.params[0].dtype == torch.float32),
+                      int(self.grads[0].dtype == torch.float32), int(self.state_bits == 8), _native.ptr(st.get("master")), st["exp_avg"].data_ptr(),
+                      st["exp_avg_sq"].data_ptr(), _native.ptr(st.get("exp_avg_scale")), _native.ptr(st.get("exp_avg_sq_scale")))
 
     @torch.no_grad()
     def refresh_masters(self) -> None:
@@ -125,19 +131,18 @@ class TensorAdamW:
         if self.device.type != "cuda":
             self.step_count += 1
             return self._step_cpu(lr, grad_scale)
-        with torch.cuda.device(self.device):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("TensorAdamW.step cannot be captured into a graph: its bias corrections follow the host's step count")
-            self.step_count += 1
-            st = self.state
-            _native.check(
-                _native.lib().ix_tensor_adamw(self._table.data_ptr(), self._chunks.data_ptr(), self._n_chunks,
-                                              int(self.params[0].dtype == torch.float32), int(self.grads[0].dtype == torch.float32),
-                                              int(self.state_bits == 8), _native.ptr(st.get("master")), st["exp_avg"].data_ptr(),
-                                              st["exp_avg_sq"].data_ptr(), _native.ptr(st.get("exp_avg_scale")),
-                                              _native.ptr(st.get("exp_avg_sq_scale")), _native.ptr(grad_scale), lr, self.betas[0],
-                                              self.betas[1], self.eps, self.step_count, _native.stream()),
-                "ix_tensor_adamw")
+        if torch.cuda.current_device() == self.device.index:
+            self._step_cuda(lr, grad_scale)
+        else:
+            with torch.cuda.device(self.device):
+                self._step_cuda(lr, grad_scale)
+
+    def _step_cuda(self, lr, grad_scale) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("TensorAdamW.step cannot be captured into a graph: its bias corrections follow the host's step count")
+        self.step_count += 1
+        _native.check(_native.lib().ix_tensor_adamw(*self._args, _native.ptr(grad_scale), lr, self.betas[0], self.betas[1], self.eps,
+                                                    self.step_count, _native.raw_stream(self.device.index)), "ix_tensor_adamw")
         torch.autograd.graph.increment_version(self.params)
 
     def _step_cpu(self, lr, grad_scale) -> None:
