@@ -1,0 +1,794 @@
+// One token per row of logits from one given number per row, with a temperature, top-k, min-p and top-p of the row's own.
+//
+// Order the tokens by logit descending, then by index ascending, with weights w_i = exp((x_i - max) / T). Keep the first k;
+// of these the ones with w >= min_p; of these the ones in front of which less than top_p of their whole weight stands (the
+// first always). The token is the one on whose stretch of the kept weight u falls. T <= 0 takes the largest logit, lowest
+// index first. The log-probability is that of the kept, renormalised distribution.
+//
+// No row is sorted. A token's weight depends on its value alone, so everything above is a search in the histogram of the
+// row's values: counts per value, weights per value in 64 bits, prefix sums over values. That keeps the sums over a whole
+// vocabulary exact to 2^-50, which a sum of 150,000 weights rounded to 32 bits is not: u falls next to a border of two
+// tokens often enough to be seen. Only values within kWindow T of the maximum count: what lies below weighs less than
+// 2^-42 of the row together, 2^-18 of the distance between two neighbouring numbers u.
+//
+// bf16 rows (sample_bf16_kernel): 16 binades of values below the largest magnitude are 4096 counters in shared memory, one
+// atomic a token. Values closer to zero (a thousandth of a row) share one more, whose weight is summed apart; a row whose
+// search ends there is marked and left to the second kernel. fp32 rows and marked ones (sample_any_kernel): 2048 equal
+// steps below the maximum with counts and weights, then the step in question digit by digit.
+//
+// Reading the row is the bound, three times (maximum, histogram, place of the token) of which two come from L2.
+#include "bw_common.cuh"
+#include "host_util.h"
+
+#include <cooperative_groups.h>
+
+namespace {
+using namespace bw;
+namespace cg = cooperative_groups;
+
+constexpr float kWindow = 42.f;       // e^-42 * 2^19 tokens < 2^-41
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+
+struct Args {
+  const void* logits;
+  long long ld;
+  int V;
+  const float* u;
+  const float* temperature;           // each may be null: 1, off, off, off
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  long long* tokens;
+  float* logprobs;
+  int* marked;                        // rows the first kernel leaves to the second (null: all rows are the second's)
+};
+
+template <typename T>
+__device__ __forceinline__ float value_of(T x);
+template <>
+__device__ __forceinline__ float value_of<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float value_of<float>(float x) { return x; }
+
+// A CTA's share of a row: 16-byte pieces [lo, hi) behind an unaligned head (rank 0) and before a tail (the last rank).
+template <typename T>
+struct Share {
+  static constexpr int kPer = 16 / sizeof(T);
+  const T* row;
+  const uint4* vec;
+  int head, lo, hi, tail0, tail1;
+  __device__ __forceinline__ Share(const Args& a, int r, int rank, int c) {
+    row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
+    head = min(a.V, off ? kPer - off : 0);
+    vec = reinterpret_cast<const uint4*>(row + head);
+    const int n = (a.V - head) / kPer;
+    lo = static_cast<int>(static_cast<long long>(n) * rank / c), hi = static_cast<int>(static_cast<long long>(n) * (rank + 1) / c);
+    tail0 = head + n * kPer, tail1 = rank == c - 1 ? a.V : tail0;
+    if (rank != 0) head = 0;          // (vec is placed already)
+    first = static_cast<int>(reinterpret_cast<const T*>(vec) - row);
+  }
+  int first;                          // index of the first element of piece 0
+  // f(value) for every element, in no particular order
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    if (static_cast<int>(threadIdx.x) < head) f(value_of<T>(row[threadIdx.x]));
+    if (tail0 + static_cast<int>(threadIdx.x) < tail1) f(value_of<T>(row[tail0 + threadIdx.x]));
+    int i = lo + threadIdx.x;
+    for (; i + 3 * kThreads < hi; i += 4 * kThreads) {
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = vec[i + q * kThreads];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) piece(w[q], f);
+    }
+    for (; i < hi; i += kThreads) piece(vec[i], f);
+  }
+  template <typename F>
+  __device__ __forceinline__ void piece(const uint4& w, F&& f) const {
+    const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) f(value_of<T>(x[q]));
+  }
+};
+
+template <typename T, typename Op>
+__device__ __forceinline__ T warp_all(T v, Op op) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+using u64 = unsigned long long;
+struct Add {
+  template <typename T>
+  __device__ T operator()(T a, T b) const { return a + b; }
+};
+
+// exclusive prefix over the block of a pair, in a fixed order; all[0..1] the totals
+template <typename A, typename B>
+__device__ __forceinline__ void block_prefix(A& x, B& y, A* sx, B* sy, A& all_x, B& all_y) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  A ix = x;
+  B iy = y;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const A ox = __shfl_up_sync(0xffffffffu, ix, d);
+    const B oy = __shfl_up_sync(0xffffffffu, iy, d);
+    if (lane >= d) ix += ox, iy += oy;
+  }
+  if (lane == 31) sx[warp] = ix, sy[warp] = iy;
+  __syncthreads();
+  A bx = 0;
+  B by = 0;
+  all_x = 0, all_y = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) bx = all_x, by = all_y;
+    all_x += sx[w], all_y += sy[w];
+  }
+  ix = __shfl_up_sync(0xffffffffu, ix, 1), iy = __shfl_up_sync(0xffffffffu, iy, 1);
+  x = bx + (lane ? ix : A(0)), y = by + (lane ? iy : B(0));
+  __syncthreads();
+}
+
+struct Row {                          // what a row asks for
+  double T, top_p, min_p, u;
+  int k;
+  bool greedy;
+  __device__ __forceinline__ Row(const Args& a, int r) {
+    const float t = a.temperature ? a.temperature[r] : 1.f;
+    greedy = !(t > 0.f);
+    T = t;
+    k = a.top_k ? a.top_k[r] : 0;
+    if (k <= 0 || k > a.V) k = a.V;
+    const float p = a.top_p ? a.top_p[r] : 1.f, m = a.min_p ? a.min_p[r] : 0.f;
+    top_p = p < 1.f ? static_cast<double>(p) : 2.0;     // 2: off (so is what is not a number)
+    min_p = m > 0.f ? static_cast<double>(m) : 0.0;
+    u = a.u[r];
+  }
+};
+
+__device__ __forceinline__ double weight(float x, float top, double T) { return x == top ? 1.0 : exp((static_cast<double>(x) - static_cast<double>(top)) / T); }
+
+struct Shared {                       // of one CTA; rank 0's copy is the cluster's
+  float top[kWarps], low[kWarps];
+  float cta_top, cta_low;
+  double sd[kWarps];
+  u64 su[kWarps];
+  unsigned sc[kWarps];
+  u64 cta_mass;
+  unsigned cta_count, cta_zero, cta_match;
+  // outcome
+  float value;
+  unsigned nth;
+  int state;                          // 1: the nth token of this value, 0: no token left, -1: marked
+  float logprob;
+  // the search's steps
+  double f0;
+  unsigned c0, c1;
+};
+
+// The row's largest value and its smallest finite one (or above -inf), over the cluster. NaN counts as -inf.
+template <typename T>
+__device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, float& top, float& low) {
+  float hi = -INFINITY, lo = INFINITY;
+  s.each([&](float x) {
+    hi = fmaxf(hi, x);
+    lo = fminf(lo, x > -INFINITY ? x : INFINITY);
+  });
+  hi = warp_all(hi, [](float a, float b) { return fmaxf(a, b); });
+  lo = warp_all(lo, [](float a, float b) { return fminf(a, b); });
+  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.top[w]), lo = fminf(lo, sh.low[w]);
+  if (c > 1) {
+    if (threadIdx.x == 0) sh.cta_top = hi, sh.cta_low = lo;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q) {
+      if (q < c) {
+        const Shared* o = cl.map_shared_rank(&sh, q);
+        hi = fmaxf(hi, o->cta_top), lo = fminf(lo, o->cta_low);
+      }
+    }
+  }
+  top = hi, low = lo;
+}
+
+// Index of the nth (from 0) element of the row that equals `value`, written by the thread that holds it. Warps own
+// neighbouring pieces, so counts in order of warp and rank are counts in order of index.
+template <typename T>
+__device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth, float logprob) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = s.hi - s.lo;
+  const int w0 = s.lo + static_cast<int>(static_cast<long long>(n) * warp / kWarps), w1 = s.lo + static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
+  auto matches = [&](int i) {         // bit q: element q of piece i
+    unsigned m = 0;
+    const uint4 w = s.vec[i];
+    const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int q = 0; q < Share<T>::kPer; ++q) m |= (value_of<T>(x[q]) == value ? 1u : 0u) << q;
+    return m;
+  };
+  unsigned mine = 0;
+#pragma unroll 4
+  for (int i = w0 + lane; i < w1; i += 32) mine += __popc(matches(i));
+  const bool is_head = warp == 0 && lane < s.head, is_tail = warp == kWarps - 1 && s.tail0 + lane < s.tail1;
+  const unsigned mh = __ballot_sync(0xffffffffu, is_head && value_of<T>(s.row[is_head ? lane : 0]) == value);
+  const unsigned mt = __ballot_sync(0xffffffffu, is_tail && value_of<T>(s.row[is_tail ? s.tail0 + lane : 0]) == value);
+  mine = warp_all(mine, Add());
+  if (lane == 0) sh.sc[warp] = mine + __popc(mh) + __popc(mt);
+  __syncthreads();
+  unsigned before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = all;
+    all += sh.sc[w];
+  }
+  if (c > 1) {
+    if (threadIdx.x == 0) sh.cta_match = all;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q)
+      if (q < rank) before += cl.map_shared_rank(&sh, q)->cta_match;
+    cl.sync();                        // nobody reaches into a peer after this
+  }
+  const unsigned here = mine + __popc(mh) + __popc(mt);
+  if (nth < before || nth >= before + here) return;
+  unsigned left = nth - before;       // of this warp's matches
+  auto nth_bit = [](unsigned m, unsigned k) {
+    for (; k; --k) m &= m - 1;
+    return __ffs(m) - 1;
+  };
+  int found = -1;
+  if (left < __popc(mh)) {
+    found = nth_bit(mh, left);
+  } else {
+    left -= __popc(mh);
+    for (int i0 = w0; i0 < w1 && found < 0; i0 += 32) {
+      const unsigned m = i0 + lane < w1 ? matches(i0 + lane) : 0u;
+      unsigned upto = __popc(m);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      const unsigned whole = __shfl_sync(0xffffffffu, upto, 31);
+      if (left < whole) {
+        const unsigned front = upto - __popc(m);
+        const bool me = left >= front && left < upto;
+        const int at = me ? s.first + (i0 + lane) * Share<T>::kPer + nth_bit(m, left - front) : 0;
+        const unsigned who = __ballot_sync(0xffffffffu, me);
+        found = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
+      } else {
+        left -= whole;
+      }
+    }
+    if (found < 0) found = s.tail0 + nth_bit(mt, left);
+  }
+  if (lane == 0) {
+    a.tokens[r] = found;
+    a.logprobs[r] = logprob;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ bf16
+constexpr int kBinades = 16, kHalf = kBinades * 128, kBins = 2 * kHalf + 1;   // negative values | around zero | positive ones
+constexpr int kEach = 2 * kHalf / kThreads;                                    // bins a thread searches
+static_assert(kEach * kThreads == 2 * kHalf, "bins are shared out evenly; the middle one goes to a thread of its own place");
+
+__global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_constant__ Args a) {
+  __shared__ unsigned bins[kBins + 3];
+  __shared__ Shared sh;
+  const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  const Share<__nv_bfloat16> s(a, r, rank, c);
+  const Row row(a, r);
+  for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
+  float top, low;
+  extremes(s, sh, c, top, low);
+  cg::cluster_group cl = cg::this_cluster();
+  if (top == -INFINITY || row.greedy) {                 // the same for the whole cluster
+    if (c > 1) cl.sync();                               // peers have read this CTA's extremes
+    if (top == -INFINITY) {
+      if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY, a.marked[r] = 0;
+      return;
+    }
+    if (rank == 0 && tid == 0) a.marked[r] = 0;
+    place(s, sh, a, r, c, rank, top, 0u, 0.f);
+    return;
+  }
+  low = top == INFINITY ? top : fmaxf(low, top - kWindow * static_cast<float>(row.T));
+  // magnitudes are compared as integers: `small` is the first one with a bin of its own
+  const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };
+  const int widest = max(mag(top), mag(low)) >> 7;
+  const int small = max(1, (widest - (kBinades - 1)) << 7), base = max(0, (widest - (kBinades - 1)) << 7);
+  unsigned zeros = 0, tiny = 0;
+  u64 tiny_mass = 0;
+  const auto one = [&](unsigned bits, unsigned n) {
+    const float x = __uint_as_float(bits << 16);
+    if (!(x >= low)) return;
+    const int m = static_cast<int>(bits & 0x7fffu);
+    if (m >= small) {
+      atomicAdd(&bins[bits & 0x8000u ? kHalf - 1 - (m - base) : kHalf + 1 + (m - base)], n);
+    } else if (m == 0) {
+      zeros += n;
+    } else {
+      tiny += n;
+      tiny_mass += n * static_cast<u64>(weight(x, top, row.T) * 17592186044416.0 + 0.5);     // 2^44
+    }
+  };
+  {
+    if (tid < s.head) one(reinterpret_cast<const unsigned short*>(s.row)[tid], 1u);
+    if (s.tail0 + tid < s.tail1) one(reinterpret_cast<const unsigned short*>(s.row)[s.tail0 + tid], 1u);
+    const auto eight = [&](const uint4& w) {
+      if (w.x == w.y && w.z == w.w && w.x == w.z && (w.x >> 16) == (w.x & 0xffffu)) {        // a mask's run: one atomic, not eight
+        one(w.x & 0xffffu, 8u);
+        return;
+      }
+      one(w.x & 0xffffu, 1u), one(w.x >> 16, 1u), one(w.y & 0xffffu, 1u), one(w.y >> 16, 1u);
+      one(w.z & 0xffffu, 1u), one(w.z >> 16, 1u), one(w.w & 0xffffu, 1u), one(w.w >> 16, 1u);
+    };
+    int i = s.lo + tid;
+    for (; i + 3 * kThreads < s.hi; i += 4 * kThreads) {
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = s.vec[i + q * kThreads];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) eight(w[q]);
+    }
+    for (; i < s.hi; i += kThreads) eight(s.vec[i]);
+  }
+  // what lies around zero, summed over the CTA
+  zeros = warp_all(zeros, Add()), tiny = warp_all(tiny, Add()), tiny_mass = warp_all(tiny_mass, Add());
+  __shared__ unsigned s_zero[kWarps], s_tiny[kWarps];
+  if ((tid & 31) == 0) s_zero[tid >> 5] = zeros, s_tiny[tid >> 5] = tiny, sh.su[tid >> 5] = tiny_mass;
+  __syncthreads();
+  if (tid == 0) {
+    unsigned z = 0, t = 0;
+    u64 m = 0;
+    for (int w = 0; w < kWarps; ++w) z += s_zero[w], t += s_tiny[w], m += sh.su[w];
+    sh.cta_zero = z, sh.cta_count = t, sh.cta_mass = m;
+  }
+  if (c > 1) {
+    cl.sync();
+    // each CTA adds up its share of the bins and puts it into rank 0's
+    unsigned* lead_bins = cl.map_shared_rank(bins, 0);
+    for (int i = kBins * rank / c + tid; i < kBins * (rank + 1) / c; i += kThreads) {
+      unsigned v[kMaxCluster], sum = 0;
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (q < c) v[q] = *cl.map_shared_rank(bins + i, q);
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (q < c) sum += v[q];
+      lead_bins[i] = sum;
+    }
+    cl.sync();
+  } else {
+    __syncthreads();
+  }
+
+  if (rank == 0) {
+    // bins in descending order of value: thread t has places kEach t .. of the 2 kHalf bins of their own; the middle one
+    // stands in front of the first negative bin, at a thread's edge
+    unsigned n[kEach];
+    double w[kEach];
+    unsigned zc = 0, tc = 0;
+    u64 tm = 0;
+    {
+      unsigned vz[kMaxCluster], vt[kMaxCluster];
+      u64 vm[kMaxCluster];
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) {
+        if (q < c) {
+          const Shared* o = cl.map_shared_rank(&sh, q);
+          vz[q] = o->cta_zero, vt[q] = o->cta_count, vm[q] = o->cta_mass;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (q < c) zc += vz[q], tc += vt[q], tm += vm[q];
+    }
+    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) + (zc ? zc * weight(0.f, top, row.T) : 0.0);
+    const unsigned mid = zc + tc;
+    const int place0 = tid * kEach;
+    const bool after_mid = place0 == kHalf;
+    const auto value_at = [&](int j) {
+      const int at = place0 + j;
+      return at < kHalf ? __uint_as_float(static_cast<unsigned>(base + kHalf - 1 - at) << 16)
+                        : __uint_as_float((0x8000u | static_cast<unsigned>(base + at - kHalf)) << 16);
+    };
+    unsigned count = after_mid ? mid : 0u;
+    double mass = after_mid ? mid_mass : 0.0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int at = place0 + j;
+      n[j] = bins[at < kHalf ? 2 * kHalf - at : 2 * kHalf - 1 - at];
+      w[j] = n[j] ? weight(value_at(j), top, row.T) : 0.0;
+      count += n[j], mass += n[j] * w[j];
+    }
+    unsigned c_all;
+    double m_all;
+    block_prefix(count, mass, sh.sc, sh.sd, c_all, m_all);
+    // now (count, mass): what stands before this thread's stretch, the middle included in front of the thread that has it.
+    // Each search ends in a number of tokens (the largest that any bin gives), and the bin that this number ends in says
+    // the weight: whole numbers, so that no rounding of a prefix leaves a search without an end, or with two
+    const unsigned c_mid = count;
+    const double m_mid = mass;
+    if (after_mid) count += mid, mass += mid_mass;
+    __shared__ int s_marked;
+    if (tid == 0) s_marked = 0, sh.c0 = 0u, sh.c1 = 1u, sh.f0 = m_all, sh.nth = 0u;
+    __syncthreads();
+    const auto weigh = [&](unsigned upto) {             // sh.f0 = weight of the first `upto` tokens
+      unsigned cc = count;
+      double mm = mass;
+      if (after_mid && mid && upto == c_mid + mid) sh.f0 = m_mid + mid_mass;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (upto > cc && upto <= cc + n[j]) sh.f0 = mm + (upto - cc) * w[j];
+        cc += n[j], mm += n[j] * w[j];
+      }
+      __syncthreads();
+      return sh.f0;
+    };
+
+    // how many tokens are kept by k and min_p, and their weight
+    unsigned keep = min(static_cast<unsigned>(row.k), c_all);
+    if (row.min_p > 0.0) {                              // tokens with w >= min_p are a prefix of the order
+      unsigned some = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) some += n[j] && w[j] >= row.min_p ? n[j] : 0u;
+      if (after_mid && mid) {
+        const float edge = __uint_as_float(static_cast<unsigned>(small) << 16);
+        if (weight(-edge, top, row.T) >= row.min_p) some += mid;
+        else if (weight(edge, top, row.T) >= row.min_p && keep > c_mid) s_marked = 1;
+      }
+      some = warp_all(some, Add());
+      if ((tid & 31) == 0) atomicAdd(&sh.c0, some);
+      __syncthreads();
+      keep = max(1u, min(keep, sh.c0));
+    }
+    if (after_mid && keep > c_mid && keep < c_mid + mid) s_marked = 1;
+    const double total = keep < c_all ? weigh(keep) : m_all;
+    // top-p: tokens in front of which less than top_p of the total stands, the first always
+    unsigned last = keep;
+    double kept = total;
+    if (row.top_p < 1.0) {
+      const double limit = row.top_p * total;
+      unsigned cc = count, upto = 1u;
+      double mm = mass;
+      if (after_mid && mid && keep > c_mid && m_mid < limit) {
+        if (m_mid + mid_mass < limit && keep >= c_mid + mid) upto = max(upto, c_mid + mid);
+        else s_marked = 1;
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const unsigned have = keep > cc ? min(n[j], keep - cc) : 0u;
+        if (have && mm < limit) upto = max(upto, cc + static_cast<unsigned>(fmin(static_cast<double>(have), fmax(ceil((limit - mm) / w[j]), 1.0))));
+        cc += n[j], mm += n[j] * w[j];
+      }
+      upto = warp_all(upto, [](unsigned x, unsigned y) { return max(x, y); });
+      if ((tid & 31) == 0) atomicMax(&sh.c1, upto);
+      __syncthreads();
+      last = sh.c1;
+      kept = weigh(last);
+    }
+    // the token: as many stand in front of it as end at or before u of the kept weight
+    {
+      const double target = row.u * kept;
+      unsigned cc = count, before = 0u;
+      double mm = mass;
+      if (after_mid && mid && last > c_mid && target >= m_mid) {
+        if (target >= m_mid + mid_mass) before = c_mid + mid;
+        else s_marked = 1;
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const unsigned have = last > cc ? min(n[j], last - cc) : 0u;
+        if (have && mm <= target) before = max(before, cc + static_cast<unsigned>(fmin(static_cast<double>(have), floor((target - mm) / w[j]))));
+        cc += n[j], mm += n[j] * w[j];
+      }
+      before = warp_all(before, [](unsigned x, unsigned y) { return max(x, y); });
+      if ((tid & 31) == 0) atomicMax(&sh.nth, before);
+      __syncthreads();
+      before = min(sh.nth, last - 1u);
+      if (tid == 0) sh.state = -1;
+      __syncthreads();                                  // everybody has read sh.nth
+      cc = count;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (before >= cc && before < cc + n[j]) {
+          sh.nth = before - cc;
+          sh.value = value_at(j);
+          sh.logprob = static_cast<float>(log(w[j] / kept));
+          sh.state = 1;
+        }
+        cc += n[j];
+      }
+      __syncthreads();
+      if (tid == 0) {
+        if (s_marked) sh.state = -1;
+        a.marked[r] = sh.state < 0;
+      }
+    }
+    __syncthreads();
+  }
+  if (c > 1) cl.sync();
+  const Shared* lead = c > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
+  const int state = lead->state;
+  const float value = lead->value, logprob = lead->logprob;
+  const unsigned nth = lead->nth;
+  if (c > 1) cl.sync();
+  if (state < 0) return;
+  place(s, sh, a, r, c, rank, value, nth, logprob);
+}
+
+// ------------------------------------------------------------------------------------------------ any type
+constexpr int kSteps = 2048, kStepsEach = kSteps / kThreads;
+constexpr double kUnit = 17592186044416.0;            // 2^44 units of weight: 2^19 tokens of weight 1 fit into 64 bits
+
+__device__ __forceinline__ unsigned order_key(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);         // -0 is 0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+struct Step {                         // what rank 0 tells the cluster
+  int go;                             // 0: this search is not needed
+  int bin;
+  unsigned prefix;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_constant__ Args a) {
+  __shared__ unsigned cnt[kSteps];
+  __shared__ u64 mas[kSteps];
+  __shared__ unsigned dcnt[256];
+  __shared__ u64 dmas[256];
+  __shared__ Shared sh;
+  __shared__ Step step[3][5];
+  const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  if (a.marked != nullptr && a.marked[r] == 0) return; // the same for the whole cluster
+  cg::cluster_group cl = cg::this_cluster();
+  const Share<T> s(a, r, rank, c);
+  const Row row(a, r);
+  for (int i = tid; i < kSteps; i += kThreads) cnt[i] = 0u, mas[i] = 0ull;
+  float top, low;
+  extremes(s, sh, c, top, low);
+  if (top == -INFINITY || row.greedy) {
+    cl.sync();
+    if (top == -INFINITY) {
+      if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY;
+      return;
+    }
+    place(s, sh, a, r, c, rank, top, 0u, 0.f);
+    return;
+  }
+  low = top == INFINITY ? top : fmaxf(low, top - kWindow * static_cast<float>(row.T));
+  // steps of a power of two, at most kSteps of them; the quotient is rounded but grows with the distance
+  const float inv = top > low ? ldexpf(1.f, 10 - ilogbf(top - low)) : 0.f;
+  const auto bin_of = [&](float x) {
+    const float q = (top - x) * inv;
+    return q < static_cast<float>(kSteps - 1) ? static_cast<int>(q) : q >= static_cast<float>(kSteps - 1) ? kSteps - 1 : 0;
+  };
+  const auto units = [&](float x) { return static_cast<u64>(weight(x, top, row.T) * kUnit + 0.5); };
+  unsigned some = 0;
+  s.each([&](float x) {
+    if (!(x >= low)) return;
+    const double w = weight(x, top, row.T);
+    const int b = bin_of(x);
+    atomicAdd(&cnt[b], 1u);
+    atomicAdd(&mas[b], static_cast<u64>(w * kUnit + 0.5));
+    some += w >= row.min_p;
+  });
+  some = warp_all(some, Add());
+  if ((tid & 31) == 0) sh.sc[tid >> 5] = some;
+  __syncthreads();
+  if (tid == 0) {
+    unsigned t = 0;
+    for (int w = 0; w < kWarps; ++w) t += sh.sc[w];
+    sh.cta_count = t;
+  }
+  cl.sync();
+  if (c > 1) {                                         // each CTA adds up its share of the steps and puts it into rank 0's
+    unsigned* lead_cnt = cl.map_shared_rank(cnt, 0);
+    u64* lead_mas = cl.map_shared_rank(mas, 0);
+    for (int i = kSteps / c * rank + tid; i < kSteps / c * (rank + 1); i += kThreads) {
+      unsigned v[kMaxCluster], x = 0;
+      u64 w[kMaxCluster], y = 0;
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (q < c) v[q] = *cl.map_shared_rank(cnt + i, q), w[q] = *cl.map_shared_rank(mas + i, q);
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (q < c) x += v[q], y += w[q];
+      lead_cnt[i] = x, lead_mas[i] = y;
+    }
+    cl.sync();
+  }
+  // rank 0 holds the cluster's histogram and its prefix sums in registers
+  unsigned n[kStepsEach], count = 0, c_all = 0, keep = 0, last = 0;
+  u64 m[kStepsEach], mass = 0, m_all = 0;
+  double total = 0.0, kept = 0.0;
+  if (rank == 0) {
+#pragma unroll
+    for (int j = 0; j < kStepsEach; ++j) {
+      n[j] = cnt[tid * kStepsEach + j], m[j] = mas[tid * kStepsEach + j];
+      count += n[j], mass += m[j];
+    }
+    unsigned fine = 0;
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q)
+      if (q < c) fine += cl.map_shared_rank(&sh, q)->cta_count;
+    block_prefix(count, mass, sh.sc, sh.su, c_all, m_all);
+    keep = max(1u, min(min(static_cast<unsigned>(row.k), c_all), fine));
+  }
+  // three searches: the kept tokens' weight (by their number), the end of top-p, the token
+  for (int what = 0; what < 3; ++what) {
+    double aim = 0.0;                                  // in units
+    if (rank == 0) {
+      if (tid == 0) step[what][0].go = what == 0 ? keep < c_all : what == 1 ? row.top_p < 1.0 : 1;
+      if (what == 0 && !(keep < c_all)) total = static_cast<double>(m_all);
+      if (what == 1) {
+        aim = row.top_p * total;
+        if (!(row.top_p < 1.0)) kept = total, last = keep;
+      }
+      if (what == 2) aim = row.u * kept;
+      __syncthreads();
+      if (step[what][0].go) {
+        // the step that the search ends in: the one with the keep-th token, the last that begins in front of the aim and
+        // among the kept ones, the last that begins at or in front of it
+        unsigned cc = count;
+        u64 mm = mass;
+#pragma unroll
+        for (int j = 0; j < kStepsEach; ++j) {
+          if (n[j]) {
+            const u64 next = mm + m[j];
+            const unsigned end = what == 2 ? last : keep;
+            bool here;
+            if (what == 0) here = cc < keep && keep <= cc + n[j];
+            else if (what == 1) here = (cc == 0 || static_cast<double>(mm) < aim) && cc < end && (!(static_cast<double>(next) < aim) || cc + n[j] >= end);
+            else here = (cc == 0 || static_cast<double>(mm) <= aim) && cc < end && (static_cast<double>(next) > aim || cc + n[j] >= end);
+            if (here) {
+              step[what][0].bin = tid * kStepsEach + j;
+              sh.c0 = cc, sh.su[0] = mm;
+            }
+          }
+          cc += n[j], mm += m[j];
+        }
+        if (tid == 0) step[what][0].prefix = 0u;
+      }
+      __syncthreads();
+    }
+    cl.sync();
+    const Step first = *cl.map_shared_rank(&step[what][0], 0);
+    if (!first.go) continue;
+    unsigned prefix = 0, seen = 0;
+    u64 weighed = 0;
+    if (rank == 0) seen = sh.c0, weighed = sh.su[0];
+    for (int level = 0; level < 4; ++level) {
+      const int shift = 24 - 8 * level;
+      if (tid < 256) dcnt[tid] = 0u, dmas[tid] = 0ull;
+      __syncthreads();
+      s.each([&](float x) {
+        if (!(x >= low) || bin_of(x) != first.bin) return;
+        const unsigned k = order_key(x);
+        if (level > 0 && (k >> (shift + 8)) != prefix) return;
+        atomicAdd(&dcnt[(k >> shift) & 255u], 1u);
+        atomicAdd(&dmas[(k >> shift) & 255u], units(x));
+      });
+      cl.sync();
+      if (rank == 0) {
+        // digits in descending order, one a thread
+        unsigned dn = 0, dc = 0, da;
+        u64 dm = 0, dw = 0, db;
+        if (tid < 256) {
+          unsigned v[kMaxCluster];
+          u64 w[kMaxCluster];
+#pragma unroll
+          for (int q = 0; q < kMaxCluster; ++q)
+            if (q < c) v[q] = *cl.map_shared_rank(dcnt + 255 - tid, q), w[q] = *cl.map_shared_rank(dmas + 255 - tid, q);
+#pragma unroll
+          for (int q = 0; q < kMaxCluster; ++q)
+            if (q < c) dn += v[q], dm += w[q];
+        }
+        dc = dn, dw = dm;
+        block_prefix(dc, dw, sh.sc, sh.su, da, db);
+        dc += seen, dw += weighed;
+        if (dn) {
+          const u64 next = dw + dm;
+          const unsigned end = what == 2 ? last : keep;
+          bool here;
+          if (what == 0) here = dc < keep && keep <= dc + dn;
+          else if (what == 1) here = (dc == 0 || static_cast<double>(dw) < aim) && dc < end && (!(static_cast<double>(next) < aim) || dc + dn >= end);
+          else here = (dc == 0 || static_cast<double>(dw) <= aim) && dc < end && (static_cast<double>(next) > aim || dc + dn >= end);
+          if (here) {
+            step[what][level + 1].prefix = (prefix << 8) | static_cast<unsigned>(255 - tid);
+            sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
+          }
+        }
+        __syncthreads();
+        seen = sh.c0, weighed = sh.cta_mass;
+      }
+      cl.sync();
+      prefix = cl.map_shared_rank(&step[what][level + 1], 0)->prefix;
+    }
+    if (rank == 0) {
+      // all tokens of one value: seen and weighed stand before them, sh.c1 is their number
+      const float x = key_value(prefix);
+      const double w = weight(x, top, row.T) * kUnit, front = static_cast<double>(weighed);
+      const unsigned end = what == 2 ? last : keep, have = min(sh.c1, end - seen);
+      if (what == 0) {
+        total = front + (keep - seen) * w;
+      } else if (what == 1) {
+        const double fit = ceil((aim - front) / w);
+        const unsigned take = static_cast<unsigned>(fmin(static_cast<double>(have), fmax(fit, 1.0)));
+        last = seen + take, kept = front + take * w;
+      } else {
+        const double at = floor((aim - front) / w);
+        if (tid == 0) {
+          sh.nth = at < 0.0 ? 0u : at < have ? static_cast<unsigned>(at) : have - 1u;
+          sh.value = x;
+          sh.logprob = static_cast<float>(log(w / kept));
+        }
+      }
+      __syncthreads();
+    }
+  }
+  cl.sync();
+  const Shared* lead = cl.map_shared_rank(&sh, 0);
+  const float value = lead->value, logprob = lead->logprob;
+  const unsigned nth = lead->nth;
+  cl.sync();
+  place(s, sh, a, r, c, rank, value, nth, logprob);
+}
+
+int launch(void (*kern)(Args), const Args& args, int rows, int cluster, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster, rows);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  IX_CUDA(cudaLaunchKernelEx(&cfg, kern, args));
+  return 0;
+}
+
+}  // namespace
+
+IX_API int ix_sample_rows_max_vocab() { return 1 << 19; }
+
+// logits [rows, V] with row stride ld, dtype 0 = bf16, 1 = fp32; u fp32 [rows] in [0, 1); temperature / top_p / min_p fp32
+// [rows], top_k int32 [rows] (each may be null); tokens int64 [rows], logprobs fp32 [rows]; marked int32 [rows] scratch (bf16).
+IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int dtype, const void* u, const void* temperature, const void* top_k,
+                          const void* top_p, const void* min_p, void* tokens, void* logprobs, void* marked, void* stream) {
+  if (rows <= 0) return 0;
+  if (rows > 65535) return ixh::fail(ixh::IX_ESIZE, "sample_rows: %d rows, at most 65535 in a call", rows);
+  if (V < 1 || V > ix_sample_rows_max_vocab()) return ixh::fail(ixh::IX_ESIZE, "sample_rows: a vocabulary of 1 to %d, not %d", ix_sample_rows_max_vocab(), V);
+  if (dtype != 0 && dtype != 1) return ixh::fail(ixh::IX_EARG, "sample_rows: dtype must be 0 (bf16) or 1 (fp32)");
+  if (dtype == 0 && marked == nullptr) return ixh::fail(ixh::IX_EARG, "sample_rows: bf16 rows need the scratch for marks");
+  Args a;
+  a.logits = logits, a.ld = ld, a.V = V;
+  a.u = static_cast<const float*>(u);
+  a.temperature = static_cast<const float*>(temperature);
+  a.top_k = static_cast<const int*>(top_k);
+  a.top_p = static_cast<const float*>(top_p);
+  a.min_p = static_cast<const float*>(min_p);
+  a.tokens = static_cast<long long*>(tokens);
+  a.logprobs = static_cast<float*>(logprobs);
+  a.marked = dtype == 0 ? static_cast<int*>(marked) : nullptr;
+  // CTAs a row: until two a multiprocessor are busy, but not beyond a few thousand tokens each
+  int c = 1;
+  while (c < kMaxCluster && rows * c < 148 * 2 && V > c * 8192) c *= 2;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, s);
+  const int rc = launch(sample_bf16_kernel, a, rows, c, s);
+  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, s);
+}

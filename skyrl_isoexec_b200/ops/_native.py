@@ -50,6 +50,8 @@ _SIGS = {
     "ix_reduce_sum": [_P, _L, _I, _I, _P, _P, _I, _P],
     "ix_clip_coef": [_P, _F, _P, _P, _P],
     "ix_adamw": [_P, _P, _P, _P, _P, _L, _I, _F, _F, _F, _F, _F, _I, _P, _P],
+    "ix_sample_rows_max_vocab": [],
+    "ix_sample_rows": [_P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "ix_lora_max_adapters": [],
     "ix_lora_max_tiles": [_I, _I, _I],
     "ix_lora_plan": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
