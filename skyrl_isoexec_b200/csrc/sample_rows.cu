@@ -20,6 +20,8 @@
 #include "bw_common.cuh"
 #include "host_util.h"
 
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 namespace {
@@ -42,6 +44,7 @@ struct Args {
   long long* tokens;
   float* logprobs;
   int* marked;                        // rows the first kernel leaves to the second (null: all rows are the second's)
+  int cached;                         // a CTA's pieces stay in shared memory after the first pass
 };
 
 template <typename T>
@@ -52,44 +55,87 @@ template <>
 __device__ __forceinline__ float value_of<float>(float x) { return x; }
 
 // A CTA's share of a row: 16-byte pieces [lo, hi) behind an unaligned head (rank 0) and before a tail (the last rank).
+extern __shared__ __align__(16) uint4 kept_pieces[];
 template <typename T>
 struct Share {
   static constexpr int kPer = 16 / sizeof(T);
   const T* row;
   const uint4* vec;
   int head, lo, hi, tail0, tail1;
+  int first;                          // index of the first element of piece 0
+  bool cached;
   __device__ __forceinline__ Share(const Args& a, int r, int rank, int c) {
     row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T));
-    head = min(a.V, off ? kPer - off : 0);
+    first = head = min(a.V, off ? kPer - off : 0);
     vec = reinterpret_cast<const uint4*>(row + head);
     const int n = (a.V - head) / kPer;
     lo = static_cast<int>(static_cast<long long>(n) * rank / c), hi = static_cast<int>(static_cast<long long>(n) * (rank + 1) / c);
     tail0 = head + n * kPer, tail1 = rank == c - 1 ? a.V : tail0;
-    if (rank != 0) head = 0;          // (vec is placed already)
-    first = static_cast<int>(reinterpret_cast<const T*>(vec) - row);
+    if (rank != 0) head = 0;
+    cached = a.cached;
   }
-  int first;                          // index of the first element of piece 0
-  // f(value) for every element, in no particular order
+  // f(element) for what is not in whole pieces
   template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    if (static_cast<int>(threadIdx.x) < head) f(value_of<T>(row[threadIdx.x]));
-    if (tail0 + static_cast<int>(threadIdx.x) < tail1) f(value_of<T>(row[tail0 + threadIdx.x]));
+  __device__ __forceinline__ void edges(F&& f) const {
+    if (static_cast<int>(threadIdx.x) < head) f(row[threadIdx.x]);
+    if (tail0 + static_cast<int>(threadIdx.x) < tail1) f(row[tail0 + threadIdx.x]);
+  }
+  // f(piece) for every piece, in no particular order; FILL: the first pass, which leaves them in shared memory
+  template <bool FILL, typename F>
+  __device__ __forceinline__ void pieces(F&& f) const {
     int i = lo + threadIdx.x;
+    if (!FILL && cached) {
+      for (; i < hi; i += kThreads) f(kept_pieces[i - lo]);
+      return;
+    }
     for (; i + 3 * kThreads < hi; i += 4 * kThreads) {
       uint4 w[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) w[q] = vec[i + q * kThreads];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) piece(w[q], f);
+      for (int q = 0; q < 4; ++q) {
+        if (FILL && cached) kept_pieces[i + q * kThreads - lo] = w[q];
+        f(w[q]);
+      }
     }
-    for (; i < hi; i += kThreads) piece(vec[i], f);
-  }
-  template <typename F>
-  __device__ __forceinline__ void piece(const uint4& w, F&& f) const {
-    const T* x = reinterpret_cast<const T*>(&w);
+    uint4 w[3];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) f(value_of<T>(x[q]));
+    for (int q = 0; q < 3; ++q)
+      if (i + q * kThreads < hi) w[q] = vec[i + q * kThreads];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      if (i + q * kThreads < hi) {
+        if (FILL && cached) kept_pieces[i + q * kThreads - lo] = w[q];
+        f(w[q]);
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 piece(int i) const { return cached ? kept_pieces[i - lo] : vec[i]; }
+  // f(value) for every element
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    edges([&](T x) { f(value_of<T>(x)); });
+    pieces<false>([&](const uint4& w) {
+      const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) f(value_of<T>(x[q]));
+    });
+  }
+  // bit q: element q of the piece equals `value`
+  __device__ __forceinline__ unsigned equal(const uint4& w, float value) const {
+    unsigned m = 0;
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 v = __float2bfloat162_rn(value);
+      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const unsigned e0 = __heq2_mask(x[0], v), e1 = __heq2_mask(x[1], v), e2 = __heq2_mask(x[2], v), e3 = __heq2_mask(x[3], v);
+      if (e0 | e1 | e2 | e3) m = (e0 & 1u) | (e0 >> 16 & 1u) << 1 | (e1 & 1u) << 2 | (e1 >> 16 & 1u) << 3 | (e2 & 1u) << 4 | (e2 >> 16 & 1u) << 5 | (e3 & 1u) << 6 | (e3 >> 16 & 1u) << 7;
+    } else {
+      const float* x = reinterpret_cast<const float*>(&w);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) m |= (x[q] == value ? 1u : 0u) << q;
+    }
+    return m;
   }
 };
 
@@ -165,18 +211,30 @@ struct Shared {                       // of one CTA; rank 0's copy is the cluste
   int state;                          // 1: the nth token of this value, 0: no token left, -1: marked
   float logprob;
   // the search's steps
-  double f0;
-  unsigned c0, c1;
+  double f0, f1;
+  unsigned c0, c1, i0;
 };
 
-// The row's largest value and its smallest finite one (or above -inf), over the cluster. NaN counts as -inf.
+// The row's largest value and its smallest one, over the cluster, without NaN; fills the kept pieces.
 template <typename T>
 __device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, float& top, float& low) {
   float hi = -INFINITY, lo = INFINITY;
-  s.each([&](float x) {
-    hi = fmaxf(hi, x);
-    lo = fminf(lo, x > -INFINITY ? x : INFINITY);
-  });
+  s.edges([&](T x) { hi = fmaxf(hi, value_of<T>(x)), lo = fminf(lo, value_of<T>(x)); });
+  if constexpr (sizeof(T) == 2) {                       // two values an instruction; the number wins over NaN
+    __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY), l = __float2bfloat162_rn(INFINITY);
+    s.template pieces<true>([&](const uint4& w) {
+      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h = __hmax2(h, x[q]), l = __hmin2(l, x[q]);
+    });
+    hi = fmaxf(hi, fmaxf(__low2float(h), __high2float(h))), lo = fminf(lo, fminf(__low2float(l), __high2float(l)));
+  } else {
+    s.template pieces<true>([&](const uint4& w) {
+      const float* x = reinterpret_cast<const float*>(&w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) hi = fmaxf(hi, x[q]), lo = fminf(lo, x[q]);
+    });
+  }
   hi = warp_all(hi, [](float a, float b) { return fmaxf(a, b); });
   lo = warp_all(lo, [](float a, float b) { return fminf(a, b); });
   if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo;
@@ -205,14 +263,7 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = s.hi - s.lo;
   const int w0 = s.lo + static_cast<int>(static_cast<long long>(n) * warp / kWarps), w1 = s.lo + static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
-  auto matches = [&](int i) {         // bit q: element q of piece i
-    unsigned m = 0;
-    const uint4 w = s.vec[i];
-    const T* x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int q = 0; q < Share<T>::kPer; ++q) m |= (value_of<T>(x[q]) == value ? 1u : 0u) << q;
-    return m;
-  };
+  auto matches = [&](int i) { return s.equal(s.piece(i), value); };
   unsigned mine = 0;
 #pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) mine += __popc(matches(i));
@@ -301,47 +352,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     place(s, sh, a, r, c, rank, top, 0u, 0.f);
     return;
   }
-  low = top == INFINITY ? top : fmaxf(low, top - kWindow * static_cast<float>(row.T));
-  // magnitudes are compared as integers: `small` is the first one with a bin of its own
+  low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
+  // magnitudes are compared as integers: `base` is the first one of the lowest binade with bins of its own. What is larger
+  // than the widest one is negative and below the window, or no number; where the widest is infinite the row is marked
   const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };
   const int widest = max(mag(top), mag(low)) >> 7;
-  const int small = max(1, (widest - (kBinades - 1)) << 7), base = max(0, (widest - (kBinades - 1)) << 7);
+  const int base = max(0, (widest - (kBinades - 1)) << 7), rare = base ? 0 : 1;
   unsigned zeros = 0, tiny = 0;
   u64 tiny_mass = 0;
-  const auto one = [&](unsigned bits, unsigned n) {
-    const float x = __uint_as_float(bits << 16);
-    if (!(x >= low)) return;
-    const int m = static_cast<int>(bits & 0x7fffu);
-    if (m >= small) {
-      atomicAdd(&bins[bits & 0x8000u ? kHalf - 1 - (m - base) : kHalf + 1 + (m - base)], n);
-    } else if (m == 0) {
-      zeros += n;
-    } else {
+  const auto around_zero = [&](unsigned bits, unsigned n) {
+    if (bits & 0x7fffu) {
       tiny += n;
-      tiny_mass += n * static_cast<u64>(weight(x, top, row.T) * 17592186044416.0 + 0.5);     // 2^44
+      tiny_mass += n * static_cast<u64>(weight(__uint_as_float(bits << 16), top, row.T) * 17592186044416.0 + 0.5);     // 2^44
+    } else {
+      zeros += n;
     }
   };
-  {
-    if (tid < s.head) one(reinterpret_cast<const unsigned short*>(s.row)[tid], 1u);
-    if (s.tail0 + tid < s.tail1) one(reinterpret_cast<const unsigned short*>(s.row)[s.tail0 + tid], 1u);
-    const auto eight = [&](const uint4& w) {
-      if (w.x == w.y && w.z == w.w && w.x == w.z && (w.x >> 16) == (w.x & 0xffffu)) {        // a mask's run: one atomic, not eight
-        one(w.x & 0xffffu, 8u);
-        return;
-      }
-      one(w.x & 0xffffu, 1u), one(w.x >> 16, 1u), one(w.y & 0xffffu, 1u), one(w.y >> 16, 1u);
-      one(w.z & 0xffffu, 1u), one(w.z >> 16, 1u), one(w.w & 0xffffu, 1u), one(w.w >> 16, 1u);
-    };
-    int i = s.lo + tid;
-    for (; i + 3 * kThreads < s.hi; i += 4 * kThreads) {
-      uint4 w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) w[q] = s.vec[i + q * kThreads];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) eight(w[q]);
+  const auto one = [&](unsigned bits) {
+    const int val = static_cast<int>(bits & 0x7fffu) - (base - 1);
+    if (val <= rare) {
+      around_zero(bits, 1u);
+    } else {
+      const unsigned bin = kHalf + (bits & 0x8000u ? -val : val);
+      if (bin < kBins) atomicAdd(&bins[bin], 1u);
     }
-    for (; i < s.hi; i += kThreads) eight(s.vec[i]);
-  }
+  };
+  s.edges([&](__nv_bfloat16 x) { one(__bfloat16_as_ushort(x)); });
+  s.pieces<false>([&](const uint4& w) {
+    if (w.x == w.y && w.z == w.w && w.x == w.z && (w.x >> 16) == (w.x & 0xffffu)) {          // a mask's run: one atomic, not eight
+      const unsigned bits = w.x & 0xffffu;
+      const int val = static_cast<int>(bits & 0x7fffu) - (base - 1);
+      const unsigned bin = kHalf + (bits & 0x8000u ? -val : val);
+      if (val <= rare) around_zero(bits, 8u);
+      else if (bin < kBins) atomicAdd(&bins[bin], 8u);
+      return;
+    }
+    one(w.x & 0xffffu), one(w.x >> 16), one(w.y & 0xffffu), one(w.y >> 16);
+    one(w.z & 0xffffu), one(w.z >> 16), one(w.w & 0xffffu), one(w.w >> 16);
+  });
   // what lies around zero, summed over the CTA
   zeros = warp_all(zeros, Add()), tiny = warp_all(tiny, Add()), tiny_mass = warp_all(tiny_mass, Add());
   __shared__ unsigned s_zero[kWarps], s_tiny[kWarps];
@@ -402,14 +450,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       return at < kHalf ? __uint_as_float(static_cast<unsigned>(base + kHalf - 1 - at) << 16)
                         : __uint_as_float((0x8000u | static_cast<unsigned>(base + at - kHalf)) << 16);
     };
-    unsigned count = after_mid ? mid : 0u;
+    unsigned count = after_mid ? mid : 0u, any = 0u;
     double mass = after_mid ? mid_mass : 0.0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int at = place0 + j;
       n[j] = bins[at < kHalf ? 2 * kHalf - at : 2 * kHalf - 1 - at];
-      w[j] = n[j] ? weight(value_at(j), top, row.T) : 0.0;
-      count += n[j], mass += n[j] * w[j];
+      any |= n[j];
+    }
+    // the thread's values are equally spaced (a binade has 128), so their weights are a geometric series
+    {
+      const float v0 = value_at(0);
+      const int e = max(1, static_cast<int>((__float_as_uint(v0) >> 23) & 255u));
+      const double ratio = any ? exp(-ldexp(1.0, e - 134) / row.T) : 0.0;
+      double run = any && v0 <= top ? weight(v0, top, row.T) : 0.0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (j) run = value_at(j) == top ? 1.0 : run * ratio;
+        w[j] = n[j] ? run : 0.0;
+        count += n[j], mass += n[j] * w[j];
+      }
     }
     unsigned c_all;
     double m_all;
@@ -443,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < kEach; ++j) some += n[j] && w[j] >= row.min_p ? n[j] : 0u;
       if (after_mid && mid) {
-        const float edge = __uint_as_float(static_cast<unsigned>(small) << 16);
+        const float edge = __uint_as_float(static_cast<unsigned>(max(1, base)) << 16);
         if (weight(-edge, top, row.T) >= row.min_p) some += mid;
         else if (weight(edge, top, row.T) >= row.min_p && keep > c_mid) s_marked = 1;
       }
@@ -468,7 +528,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         const unsigned have = keep > cc ? min(n[j], keep - cc) : 0u;
-        if (have && mm < limit) upto = max(upto, cc + static_cast<unsigned>(fmin(static_cast<double>(have), fmax(ceil((limit - mm) / w[j]), 1.0))));
+        if (have && mm < limit) {
+          const bool through = mm + have * w[j] < limit;
+          upto = max(upto, cc + (through ? have : static_cast<unsigned>(fmin(static_cast<double>(have), fmax(ceil((limit - mm) / w[j]), 1.0)))));
+        }
         cc += n[j], mm += n[j] * w[j];
       }
       upto = warp_all(upto, [](unsigned x, unsigned y) { return max(x, y); });
@@ -479,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     }
     // the token: as many stand in front of it as end at or before u of the kept weight
     {
+      if (tid == kThreads - 32) sh.f1 = log(kept);       // beside the search
       const double target = row.u * kept;
       unsigned cc = count, before = 0u;
       double mm = mass;
@@ -489,7 +553,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         const unsigned have = last > cc ? min(n[j], last - cc) : 0u;
-        if (have && mm <= target) before = max(before, cc + static_cast<unsigned>(fmin(static_cast<double>(have), floor((target - mm) / w[j]))));
+        if (have && mm <= target) {
+          const bool past = mm + have * w[j] <= target;
+          before = max(before, cc + (past ? have : static_cast<unsigned>(fmin(static_cast<double>(have), floor((target - mm) / w[j])))));
+        }
         cc += n[j], mm += n[j] * w[j];
       }
       before = warp_all(before, [](unsigned x, unsigned y) { return max(x, y); });
@@ -504,14 +571,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
         if (before >= cc && before < cc + n[j]) {
           sh.nth = before - cc;
           sh.value = value_at(j);
-          sh.logprob = static_cast<float>(log(w[j] / kept));
+          sh.logprob = static_cast<float>((static_cast<double>(sh.value) - static_cast<double>(top)) / row.T - sh.f1);
           sh.state = 1;
         }
         cc += n[j];
       }
       __syncthreads();
       if (tid == 0) {
-        if (s_marked) sh.state = -1;
+        if (s_marked || widest == 255) sh.state = -1;
         a.marked[r] = sh.state < 0;
       }
     }
@@ -540,8 +607,28 @@ __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(
 struct Step {                         // what rank 0 tells the cluster
   int go;                             // 0: this search is not needed
   int bin;
+  int few;                            // the bin's tokens fit into the list
   unsigned prefix;
 };
+constexpr int kList = 1024;
+// Whether a search ends in the n tokens that stand behind cc others (weights in units: mm before them, next behind them).
+// 0: the end-th token. 1: the last that begin in front of the aim and among the first `end`. 2: the last that begin at or
+// in front of it. Exactly one of a row's bins, or of a bin's values, says yes: the sums are whole numbers.
+__device__ __forceinline__ bool here(int what, unsigned cc, unsigned n, u64 mm, u64 next, double aim, unsigned end) {
+  if (what == 0) return cc < end && end <= cc + n;
+  if (what == 1) return (cc == 0 || static_cast<double>(mm) < aim) && cc < end && (!(static_cast<double>(next) < aim) || cc + n >= end);
+  return (cc == 0 || static_cast<double>(mm) <= aim) && cc < end && (static_cast<double>(next) > aim || cc + n >= end);
+}
+
+// exp(-t / log2 e) in units, t >= 0: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven
+// implementation of the exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits
+__device__ __forceinline__ u64 units_of(double t, const double* table) {
+  if (!(t < 64.0)) return 0ull;                        // below 2^-64: nothing in units of 2^-44
+  const int n = static_cast<int>(t * 64.0);
+  const double f = (t - n * (1.0 / 64.0)) * -0.69314718055994530942;
+  const double e = 1.0 + f * (1.0 + f * (1.0 / 2 + f * (1.0 / 6 + f * (1.0 / 24 + f * (1.0 / 120)))));
+  return static_cast<u64>(e * __longlong_as_double(__double_as_longlong(table[n & 63]) - (static_cast<long long>(n >> 6) << 52)) + 0.5);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_constant__ Args a) {
@@ -551,12 +638,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   __shared__ u64 dmas[256];
   __shared__ Shared sh;
   __shared__ Step step[3][5];
+  __shared__ unsigned list[kList], list_n;
+  __shared__ double table[64];        // 2^(44 - i / 64)
   const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   if (a.marked != nullptr && a.marked[r] == 0) return; // the same for the whole cluster
   cg::cluster_group cl = cg::this_cluster();
   const Share<T> s(a, r, rank, c);
   const Row row(a, r);
   for (int i = tid; i < kSteps; i += kThreads) cnt[i] = 0u, mas[i] = 0ull;
+  if (tid < 64) table[tid] = exp2(44.0 - tid / 64.0);
   float top, low;
   extremes(s, sh, c, top, low);
   if (top == -INFINITY || row.greedy) {
@@ -568,22 +658,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     place(s, sh, a, r, c, rank, top, 0u, 0.f);
     return;
   }
-  low = top == INFINITY ? top : fmaxf(low, top - kWindow * static_cast<float>(row.T));
+  low = top == INFINITY ? top : fmaxf(fmaxf(low, -FLT_MAX), top - kWindow * static_cast<float>(row.T));
   // steps of a power of two, at most kSteps of them; the quotient is rounded but grows with the distance
   const float inv = top > low ? ldexpf(1.f, 10 - ilogbf(top - low)) : 0.f;
   const auto bin_of = [&](float x) {
     const float q = (top - x) * inv;
     return q < static_cast<float>(kSteps - 1) ? static_cast<int>(q) : q >= static_cast<float>(kSteps - 1) ? kSteps - 1 : 0;
   };
-  const auto units = [&](float x) { return static_cast<u64>(weight(x, top, row.T) * kUnit + 0.5); };
+  const double per = 1.4426950408889634 / row.T;
+  const auto units = [&](float x) { return x == top ? static_cast<u64>(kUnit) : units_of((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
+  const double floor_units = row.min_p * kUnit;
   unsigned some = 0;
   s.each([&](float x) {
     if (!(x >= low)) return;
-    const double w = weight(x, top, row.T);
+    const u64 q = units(x);
     const int b = bin_of(x);
     atomicAdd(&cnt[b], 1u);
-    atomicAdd(&mas[b], static_cast<u64>(w * kUnit + 0.5));
-    some += w >= row.min_p;
+    atomicAdd(&mas[b], q);
+    // on the border itself (a unit is 2^-44) the weight decides
+    if (row.min_p > 0.0) some += fabs(static_cast<double>(q) - floor_units) > 2.0 ? static_cast<double>(q) > floor_units : weight(x, top, row.T) >= row.min_p;
+    else ++some;
   });
   some = warp_all(some, Add());
   if ((tid & 31) == 0) sh.sc[tid >> 5] = some;
@@ -640,27 +734,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       if (what == 2) aim = row.u * kept;
       __syncthreads();
       if (step[what][0].go) {
-        // the step that the search ends in: the one with the keep-th token, the last that begins in front of the aim and
-        // among the kept ones, the last that begins at or in front of it
         unsigned cc = count;
         u64 mm = mass;
 #pragma unroll
         for (int j = 0; j < kStepsEach; ++j) {
           if (n[j]) {
-            const u64 next = mm + m[j];
-            const unsigned end = what == 2 ? last : keep;
-            bool here;
-            if (what == 0) here = cc < keep && keep <= cc + n[j];
-            else if (what == 1) here = (cc == 0 || static_cast<double>(mm) < aim) && cc < end && (!(static_cast<double>(next) < aim) || cc + n[j] >= end);
-            else here = (cc == 0 || static_cast<double>(mm) <= aim) && cc < end && (static_cast<double>(next) > aim || cc + n[j] >= end);
-            if (here) {
+            if (here(what, cc, n[j], mm, mm + m[j], aim, what == 2 ? last : keep)) {
               step[what][0].bin = tid * kStepsEach + j;
+              step[what][0].few = n[j] <= kList;
               sh.c0 = cc, sh.su[0] = mm;
             }
           }
           cc += n[j], mm += m[j];
         }
-        if (tid == 0) step[what][0].prefix = 0u;
+        if (tid == 0) list_n = 0u;
       }
       __syncthreads();
     }
@@ -670,7 +757,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     unsigned prefix = 0, seen = 0;
     u64 weighed = 0;
     if (rank == 0) seen = sh.c0, weighed = sh.su[0];
-    for (int level = 0; level < 4; ++level) {
+    if (first.few) {
+      // the bin's tokens in a list of rank 0; each finds what stands in front of it by looking at all the others
+      unsigned* to = cl.map_shared_rank(list, 0);
+      unsigned* at = cl.map_shared_rank(&list_n, 0);
+      s.each([&](float x) {
+        if (x >= low && bin_of(x) == first.bin) to[atomicAdd(at, 1u)] = order_key(x);
+      });
+      cl.sync();
+      if (rank == 0) {
+        const unsigned many = list_n;
+        for (unsigned i = tid; i < many; i += kThreads) {
+          const unsigned k = list[i];
+          unsigned dc = seen, dn = 0u;
+          u64 dw = weighed;
+          const u64 q = units(key_value(k));
+          for (unsigned j = 0; j < many; ++j) {
+            const unsigned o = list[j];
+            if (o > k) ++dc, dw += units(key_value(o));
+            dn += o == k;
+          }
+          if (here(what, dc, dn, dw, dw + dn * q, aim, what == 2 ? last : keep)) sh.i0 = k, sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
+        }
+        __syncthreads();
+        prefix = sh.i0, seen = sh.c0, weighed = sh.cta_mass;
+      }
+    }
+    for (int level = 0; level < 4 && !first.few; ++level) {
       const int shift = 24 - 8 * level;
       if (tid < 256) dcnt[tid] = 0u, dmas[tid] = 0ull;
       __syncthreads();
@@ -700,13 +813,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         block_prefix(dc, dw, sh.sc, sh.su, da, db);
         dc += seen, dw += weighed;
         if (dn) {
-          const u64 next = dw + dm;
-          const unsigned end = what == 2 ? last : keep;
-          bool here;
-          if (what == 0) here = dc < keep && keep <= dc + dn;
-          else if (what == 1) here = (dc == 0 || static_cast<double>(dw) < aim) && dc < end && (!(static_cast<double>(next) < aim) || dc + dn >= end);
-          else here = (dc == 0 || static_cast<double>(dw) <= aim) && dc < end && (static_cast<double>(next) > aim || dc + dn >= end);
-          if (here) {
+          if (here(what, dc, dn, dw, dw + dm, aim, what == 2 ? last : keep)) {
             step[what][level + 1].prefix = (prefix << 8) | static_cast<unsigned>(255 - tid);
             sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
           }
@@ -721,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       // all tokens of one value: seen and weighed stand before them, sh.c1 is their number
       const float x = key_value(prefix);
       const double w = weight(x, top, row.T) * kUnit, front = static_cast<double>(weighed);
-      const unsigned end = what == 2 ? last : keep, have = min(sh.c1, end - seen);
+      const unsigned have = min(sh.c1, (what == 2 ? last : keep) - seen);
       if (what == 0) {
         total = front + (keep - seen) * w;
       } else if (what == 1) {
@@ -747,8 +854,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   place(s, sh, a, r, c, rank, value, nth, logprob);
 }
 
-int launch(void (*kern)(Args), const Args& args, int rows, int cluster, cudaStream_t s) {
+int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem, cudaStream_t s) {
+  if (smem > 16 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = dim3(cluster, rows);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
@@ -784,11 +893,15 @@ IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int
   a.tokens = static_cast<long long*>(tokens);
   a.logprobs = static_cast<float*>(logprobs);
   a.marked = dtype == 0 ? static_cast<int*>(marked) : nullptr;
-  // CTAs a row: until two a multiprocessor are busy, but not beyond a few thousand tokens each
+  // CTAs a row: as many as leave all rows' CTAs resident together (two a multiprocessor), but not beyond a few thousand
+  // tokens each. Where its pieces then fit beside another CTA's, they stay in shared memory after the first pass
   int c = 1;
-  while (c < kMaxCluster && rows * c < 148 * 2 && V > c * 8192) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= 148 * 2 && V > c * 8192) c *= 2;
+  const long long bytes = (static_cast<long long>(V) * (dtype == 0 ? 2 : 4) / c + 32 + 15) / 16 * 16;
+  a.cached = bytes <= 72 * 1024;
+  const int smem = a.cached ? static_cast<int>(bytes) : 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, s);
-  const int rc = launch(sample_bf16_kernel, a, rows, c, s);
-  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, s);
+  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, smem, s);
+  const int rc = launch(sample_bf16_kernel, a, rows, c, smem, s);
+  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, smem, s);
 }
