@@ -197,6 +197,19 @@ struct Row {                          // what a row asks for
 
 __device__ __forceinline__ double weight(float x, float top, double T) { return x == top ? 1.0 : exp((static_cast<double>(x) - static_cast<double>(top)) / T); }
 
+// 2^-t for t >= 0: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven implementation of the
+// exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits, good to 1e-14
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x * (-1.0 / 64.0));
+}
+__device__ __forceinline__ double two_to_minus(double t, const double* table) {
+  if (!(t < 900.0)) return 0.0;
+  const int n = static_cast<int>(t * 64.0);
+  const double f = (t - n * (1.0 / 64.0)) * -0.69314718055994530942;
+  const double e = 1.0 + f * (1.0 + f * (1.0 / 2 + f * (1.0 / 6 + f * (1.0 / 24 + f * (1.0 / 120)))));
+  return e * __longlong_as_double(__double_as_longlong(table[n & 63]) - (static_cast<long long>(n >> 6) << 52));
+}
+
 struct Shared {                       // of one CTA; rank 0's copy is the cluster's
   float top[kWarps], low[kWarps];
   float cta_top, cta_low;
@@ -209,7 +222,6 @@ struct Shared {                       // of one CTA; rank 0's copy is the cluste
   float value;
   unsigned nth;
   int state;                          // 1: the nth token of this value, 0: no token left, -1: marked
-  float logprob;
   // the search's steps
   double f0, f1;
   unsigned c0, c1, i0;
@@ -256,17 +268,30 @@ __device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, f
   top = hi, low = lo;
 }
 
-// Index of the nth (from 0) element of the row that equals `value`, written by the thread that holds it. Warps own
-// neighbouring pieces, so counts in order of warp and rank are counts in order of index.
+// Writes the row's outcome: the index of the nth (from 0) element that equals `value`, by the warp that holds it, and the
+// log-probability (value - top) / T - log(kept), by a warp of rank 0 beside it. Warps own neighbouring pieces, so counts in
+// order of warp and rank are counts in order of index.
 template <typename T>
-__device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth, float logprob) {
+__device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth, float top,
+                                      double temperature, double kept) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = s.hi - s.lo;
   const int w0 = s.lo + static_cast<int>(static_cast<long long>(n) * warp / kWarps), w1 = s.lo + static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
   auto matches = [&](int i) { return s.equal(s.piece(i), value); };
   unsigned mine = 0;
-#pragma unroll 4
-  for (int i = w0 + lane; i < w1; i += 32) mine += __popc(matches(i));
+  if (s.cached) {
+    for (int i = w0 + lane; i < w1; i += 32) mine += __popc(s.equal(kept_pieces[i - s.lo], value));
+  } else {
+    int i = w0 + lane;
+    for (; i + 7 * 32 < w1; i += 8 * 32) {
+      uint4 w[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) w[q] = s.vec[i + q * 32];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) mine += __popc(s.equal(w[q], value));
+    }
+    for (; i < w1; i += 32) mine += __popc(s.equal(s.vec[i], value));
+  }
   const bool is_head = warp == 0 && lane < s.head, is_tail = warp == kWarps - 1 && s.tail0 + lane < s.tail1;
   const unsigned mh = __ballot_sync(0xffffffffu, is_head && value_of<T>(s.row[is_head ? lane : 0]) == value);
   const unsigned mt = __ballot_sync(0xffffffffu, is_tail && value_of<T>(s.row[is_tail ? s.tail0 + lane : 0]) == value);
@@ -283,11 +308,17 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
     if (threadIdx.x == 0) sh.cta_match = all;
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
+    unsigned v[kMaxCluster];
 #pragma unroll
     for (int q = 0; q < kMaxCluster; ++q)
-      if (q < rank) before += cl.map_shared_rank(&sh, q)->cta_match;
+      if (q < rank) v[q] = cl.map_shared_rank(&sh, q)->cta_match;
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q)
+      if (q < rank) before += v[q];
     cl.sync();                        // nobody reaches into a peer after this
   }
+  if (rank == 0 && threadIdx.x == kThreads - 1)
+    a.logprobs[r] = static_cast<float>((value == top ? 0.0 : (static_cast<double>(value) - static_cast<double>(top)) / temperature) - log(kept));
   const unsigned here = mine + __popc(mh) + __popc(mt);
   if (nth < before || nth >= before + here) return;
   unsigned left = nth - before;       // of this warp's matches
@@ -321,10 +352,7 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
     }
     if (found < 0) found = s.tail0 + nth_bit(mt, left);
   }
-  if (lane == 0) {
-    a.tokens[r] = found;
-    a.logprobs[r] = logprob;
-  }
+  if (lane == 0) a.tokens[r] = found;
 }
 
 // ------------------------------------------------------------------------------------------------ bf16
@@ -334,11 +362,14 @@ static_assert(kEach * kThreads == 2 * kHalf, "bins are shared out evenly; the mi
 
 __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_constant__ Args a) {
   __shared__ unsigned bins[kBins + 3];
+  __shared__ double table[64];
   __shared__ Shared sh;
   const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  pdl_launch_dependents();
   const Share<__nv_bfloat16> s(a, r, rank, c);
   const Row row(a, r);
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
+  fill_table(table);
   float top, low;
   extremes(s, sh, c, top, low);
   cg::cluster_group cl = cg::this_cluster();
@@ -349,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       return;
     }
     if (rank == 0 && tid == 0) a.marked[r] = 0;
-    place(s, sh, a, r, c, rank, top, 0u, 0.f);
+    place(s, sh, a, r, c, rank, top, 0u, top, 1.0, 1.0);
     return;
   }
   low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
@@ -357,38 +388,48 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   // than the widest one is negative and below the window, or no number; where the widest is infinite the row is marked
   const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };
   const int widest = max(mag(top), mag(low)) >> 7;
-  const int base = max(0, (widest - (kBinades - 1)) << 7), rare = base ? 0 : 1;
+  const int base = max(0, (widest - (kBinades - 1)) << 7), first = max(1, base);
+  const double per = 1.4426950408889634 / row.T;
+  const auto weigh_value = [&](float x) { return x == top ? 1.0 : two_to_minus((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
   unsigned zeros = 0, tiny = 0;
   u64 tiny_mass = 0;
   const auto around_zero = [&](unsigned bits, unsigned n) {
     if (bits & 0x7fffu) {
+      const float x = __uint_as_float(bits << 16);
       tiny += n;
-      tiny_mass += n * static_cast<u64>(weight(__uint_as_float(bits << 16), top, row.T) * 17592186044416.0 + 0.5);     // 2^44
+      if (x >= low) tiny_mass += n * static_cast<u64>(weigh_value(x) * 17592186044416.0 + 0.5);     // 2^44
     } else {
       zeros += n;
     }
   };
-  const auto one = [&](unsigned bits) {
-    const int val = static_cast<int>(bits & 0x7fffu) - (base - 1);
-    if (val <= rare) {
-      around_zero(bits, 1u);
-    } else {
-      const unsigned bin = kHalf + (bits & 0x8000u ? -val : val);
-      if (bin < kBins) atomicAdd(&bins[bin], 1u);
-    }
+  // distance from the first magnitude with a bin: less than kHalf of them have one, a negative distance is around zero
+  const unsigned some = kHalf + base - first;
+  unsigned* const up = bins + kHalf + 1 + (first - base);
+  unsigned* const downward = bins + kHalf - (first - base);        // one past the first negative bin: -d is ~d + 1
+  const auto add = [&](unsigned bits, unsigned n) {
+    const int d = static_cast<int>(bits & 0x7fffu) - first;
+    const int sign = -static_cast<int>(bits >> 15 & 1u);
+    if (static_cast<unsigned>(d) < some) atomicAdd((sign ? downward : up) + (d ^ sign), n);
+    return d;
   };
-  s.edges([&](__nv_bfloat16 x) { one(__bfloat16_as_ushort(x)); });
+  s.edges([&](__nv_bfloat16 x) {
+    const unsigned bits = __bfloat16_as_ushort(x);
+    if (add(bits, 1u) < 0) around_zero(bits, 1u);
+  });
   s.pieces<false>([&](const uint4& w) {
     if (w.x == w.y && w.z == w.w && w.x == w.z && (w.x >> 16) == (w.x & 0xffffu)) {          // a mask's run: one atomic, not eight
-      const unsigned bits = w.x & 0xffffu;
-      const int val = static_cast<int>(bits & 0x7fffu) - (base - 1);
-      const unsigned bin = kHalf + (bits & 0x8000u ? -val : val);
-      if (val <= rare) around_zero(bits, 8u);
-      else if (bin < kBins) atomicAdd(&bins[bin], 8u);
+      if (add(w.x & 0xffffu, 8u) < 0) around_zero(w.x & 0xffffu, 8u);
       return;
     }
-    one(w.x & 0xffffu), one(w.x >> 16), one(w.y & 0xffffu), one(w.y >> 16);
-    one(w.z & 0xffffu), one(w.z >> 16), one(w.w & 0xffffu), one(w.w >> 16);
+    int below = add(w.x & 0xffffu, 1u) | add(w.x >> 16, 1u) | add(w.y & 0xffffu, 1u) | add(w.y >> 16, 1u);
+    below |= add(w.z & 0xffffu, 1u) | add(w.z >> 16, 1u) | add(w.w & 0xffffu, 1u) | add(w.w >> 16, 1u);
+    if (below < 0) {
+#pragma unroll 1
+      for (int q = 0; q < 8; ++q) {
+        const unsigned word = q < 4 ? (q < 2 ? w.x : w.y) : (q < 6 ? w.z : w.w), bits = q & 1 ? word >> 16 : word & 0xffffu;
+        if (static_cast<int>(bits & 0x7fffu) < first) around_zero(bits, 1u);
+      }
+    }
   });
   // what lies around zero, summed over the CTA
   zeros = warp_all(zeros, Add()), tiny = warp_all(tiny, Add()), tiny_mass = warp_all(tiny_mass, Add());
@@ -441,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       for (int q = 0; q < kMaxCluster; ++q)
         if (q < c) zc += vz[q], tc += vt[q], tm += vm[q];
     }
-    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) + (zc ? zc * weight(0.f, top, row.T) : 0.0);
+    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) + (zc ? zc * weigh_value(0.f) : 0.0);
     const unsigned mid = zc + tc;
     const int place0 = tid * kEach;
     const bool after_mid = place0 == kHalf;
@@ -462,8 +503,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     {
       const float v0 = value_at(0);
       const int e = max(1, static_cast<int>((__float_as_uint(v0) >> 23) & 255u));
-      const double ratio = any ? exp(-ldexp(1.0, e - 134) / row.T) : 0.0;
-      double run = any && v0 <= top ? weight(v0, top, row.T) : 0.0;
+      const double ratio = any ? two_to_minus(__longlong_as_double(static_cast<long long>(e - 134 + 1023) << 52) * per, table) : 0.0;
+      double run = any && v0 <= top ? weigh_value(v0) : 0.0;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         if (j) run = value_at(j) == top ? 1.0 : run * ratio;
@@ -504,8 +545,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       for (int j = 0; j < kEach; ++j) some += n[j] && w[j] >= row.min_p ? n[j] : 0u;
       if (after_mid && mid) {
         const float edge = __uint_as_float(static_cast<unsigned>(max(1, base)) << 16);
-        if (weight(-edge, top, row.T) >= row.min_p) some += mid;
-        else if (weight(edge, top, row.T) >= row.min_p && keep > c_mid) s_marked = 1;
+        if (weigh_value(-edge) >= row.min_p) some += mid;
+        else if ((edge >= top || weigh_value(edge) >= row.min_p) && keep > c_mid) s_marked = 1;
       }
       some = warp_all(some, Add());
       if ((tid & 31) == 0) atomicAdd(&sh.c0, some);
@@ -542,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     }
     // the token: as many stand in front of it as end at or before u of the kept weight
     {
-      if (tid == kThreads - 32) sh.f1 = log(kept);       // beside the search
+      if (tid == 0) sh.f1 = kept;
       const double target = row.u * kept;
       unsigned cc = count, before = 0u;
       double mm = mass;
@@ -571,7 +612,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
         if (before >= cc && before < cc + n[j]) {
           sh.nth = before - cc;
           sh.value = value_at(j);
-          sh.logprob = static_cast<float>((static_cast<double>(sh.value) - static_cast<double>(top)) / row.T - sh.f1);
           sh.state = 1;
         }
         cc += n[j];
@@ -587,11 +627,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   if (c > 1) cl.sync();
   const Shared* lead = c > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
   const int state = lead->state;
-  const float value = lead->value, logprob = lead->logprob;
+  const float value = lead->value;
   const unsigned nth = lead->nth;
-  if (c > 1) cl.sync();
-  if (state < 0) return;
-  place(s, sh, a, r, c, rank, value, nth, logprob);
+  const double kept_mass = lead->f1;
+  if (state < 0) {
+    if (c > 1) cl.sync();               // peers have read this CTA's outcome
+    return;
+  }
+  place(s, sh, a, r, c, rank, value, nth, top, row.T, kept_mass);
 }
 
 // ------------------------------------------------------------------------------------------------ any type
@@ -620,14 +663,8 @@ __device__ __forceinline__ bool here(int what, unsigned cc, unsigned n, u64 mm, 
   return (cc == 0 || static_cast<double>(mm) <= aim) && cc < end && (static_cast<double>(next) > aim || cc + n >= end);
 }
 
-// exp(-t / log2 e) in units, t >= 0: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven
-// implementation of the exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits
 __device__ __forceinline__ u64 units_of(double t, const double* table) {
-  if (!(t < 64.0)) return 0ull;                        // below 2^-64: nothing in units of 2^-44
-  const int n = static_cast<int>(t * 64.0);
-  const double f = (t - n * (1.0 / 64.0)) * -0.69314718055994530942;
-  const double e = 1.0 + f * (1.0 + f * (1.0 / 2 + f * (1.0 / 6 + f * (1.0 / 24 + f * (1.0 / 120)))));
-  return static_cast<u64>(e * __longlong_as_double(__double_as_longlong(table[n & 63]) - (static_cast<long long>(n >> 6) << 52)) + 0.5);
+  return t < 64.0 ? static_cast<u64>(two_to_minus(t, table) * kUnit + 0.5) : 0ull;      // nothing in units of 2^-44
 }
 
 template <typename T>
@@ -639,14 +676,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   __shared__ Shared sh;
   __shared__ Step step[3][5];
   __shared__ unsigned list[kList], list_n;
-  __shared__ double table[64];        // 2^(44 - i / 64)
+  __shared__ double table[64];
   const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
-  if (a.marked != nullptr && a.marked[r] == 0) return; // the same for the whole cluster
+  if (a.marked != nullptr) {
+    pdl_wait();
+    if (a.marked[r] == 0) return;                      // the same for the whole cluster
+  }
   cg::cluster_group cl = cg::this_cluster();
   const Share<T> s(a, r, rank, c);
   const Row row(a, r);
   for (int i = tid; i < kSteps; i += kThreads) cnt[i] = 0u, mas[i] = 0ull;
-  if (tid < 64) table[tid] = exp2(44.0 - tid / 64.0);
+  fill_table(table);
   float top, low;
   extremes(s, sh, c, top, low);
   if (top == -INFINITY || row.greedy) {
@@ -655,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY;
       return;
     }
-    place(s, sh, a, r, c, rank, top, 0u, 0.f);
+    place(s, sh, a, r, c, rank, top, 0u, top, 1.0, 1.0);
     return;
   }
   low = top == INFINITY ? top : fmaxf(fmaxf(low, -FLT_MAX), top - kWindow * static_cast<float>(row.T));
@@ -840,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         if (tid == 0) {
           sh.nth = at < 0.0 ? 0u : at < have ? static_cast<unsigned>(at) : have - 1u;
           sh.value = x;
-          sh.logprob = static_cast<float>(log(w / kept));
+          sh.f1 = kept / kUnit;
         }
       }
       __syncthreads();
@@ -848,24 +888,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   }
   cl.sync();
   const Shared* lead = cl.map_shared_rank(&sh, 0);
-  const float value = lead->value, logprob = lead->logprob;
+  const float value = lead->value;
   const unsigned nth = lead->nth;
-  cl.sync();
-  place(s, sh, a, r, c, rank, value, nth, logprob);
+  const double kept_mass = lead->f1;
+  place(s, sh, a, r, c, rank, value, nth, top, row.T, kept_mass);
 }
 
-int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem, cudaStream_t s) {
+int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem, bool early, cudaStream_t s) {
   if (smem > 16 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = smem;
   cfg.gridDim = dim3(cluster, rows);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early && ixh::pdl_enabled() ? 2 : 1;
   IX_CUDA(cudaLaunchKernelEx(&cfg, kern, args));
   return 0;
 }
@@ -901,7 +943,8 @@ IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int
   a.cached = bytes <= 72 * 1024;
   const int smem = a.cached ? static_cast<int>(bytes) : 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, smem, s);
-  const int rc = launch(sample_bf16_kernel, a, rows, c, smem, s);
-  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, smem, s);
+  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, smem, false, s);
+  const int rc = launch(sample_bf16_kernel, a, rows, c, smem, false, s);
+  // started while the first one drains: it waits for its marks, and nearly always ends there
+  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, smem, true, s);
 }
