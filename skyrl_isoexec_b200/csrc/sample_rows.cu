@@ -220,11 +220,13 @@ struct Shared {                       // of one CTA; rank 0's copy is the cluste
   unsigned cta_count, cta_zero, cta_match;
   // outcome
   float value;
-  unsigned nth;
+  unsigned nth, ties;
   int state;                          // 1: the nth token of this value, 0: no token left, -1: marked
   // the search's steps
   double f0, f1;
   unsigned c0, c1, i0;
+  // what place() finds
+  unsigned found_n, found_min;
 };
 
 // The row's largest value and its smallest one, over the cluster, without NaN; fills the kept pieces.
@@ -268,12 +270,10 @@ __device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, f
   top = hi, low = lo;
 }
 
-// Writes the row's outcome: the index of the nth (from 0) element that equals `value`, by the warp that holds it, and the
-// log-probability (value - top) / T - log(kept), by a warp of rank 0 beside it. Warps own neighbouring pieces, so counts in
-// order of warp and rank are counts in order of index.
+// Index of the nth (from 0) element that equals `value`, for any number of them: warps own neighbouring pieces, so counts in
+// order of warp and rank are counts in order of index. Out of line: rows with that many equal values are rare.
 template <typename T>
-__device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth, float top,
-                                      double temperature, double kept) {
+__device__ __noinline__ void place_among_many(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = s.hi - s.lo;
   const int w0 = s.lo + static_cast<int>(static_cast<long long>(n) * warp / kWarps), w1 = s.lo + static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
@@ -317,8 +317,6 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
       if (q < rank) before += v[q];
     cl.sync();                        // nobody reaches into a peer after this
   }
-  if (rank == 0 && threadIdx.x == kThreads - 1)
-    a.logprobs[r] = static_cast<float>((value == top ? 0.0 : (static_cast<double>(value) - static_cast<double>(top)) / temperature) - log(kept));
   const unsigned here = mine + __popc(mh) + __popc(mt);
   if (nth < before || nth >= before + here) return;
   unsigned left = nth - before;       // of this warp's matches
@@ -331,28 +329,108 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
     found = nth_bit(mh, left);
   } else {
     left -= __popc(mh);
-    for (int i0 = w0; i0 < w1 && found < 0; i0 += 32) {
-      const unsigned m = i0 + lane < w1 ? matches(i0 + lane) : 0u;
-      unsigned upto = __popc(m);
+    for (int i0 = w0; i0 < w1 && found < 0; i0 += 8 * 32) {
+      unsigned m[8], all8 = 0;        // 8 x 32 pieces at a time: one wait for all of them
+#pragma unroll
+      for (int q = 0; q < 8; ++q) m[q] = i0 + q * 32 + lane < w1 ? matches(i0 + q * 32 + lane) : 0u;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) all8 += __popc(m[q]);
+      all8 = warp_all(all8, Add());
+      if (left >= all8) {
+        left -= all8;
+        continue;
+      }
+      unsigned mine8 = 0;             // the eighth that has it
+      int eighth = 0;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const unsigned whole = warp_all(static_cast<unsigned>(__popc(m[q])), Add());
+        if (eighth == q) {
+          mine8 = m[q];
+          if (left >= whole) left -= whole, ++eighth;
+        }
+      }
+      unsigned upto = __popc(mine8);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += o;
       }
-      const unsigned whole = __shfl_sync(0xffffffffu, upto, 31);
-      if (left < whole) {
-        const unsigned front = upto - __popc(m);
-        const bool me = left >= front && left < upto;
-        const int at = me ? s.first + (i0 + lane) * Share<T>::kPer + nth_bit(m, left - front) : 0;
-        const unsigned who = __ballot_sync(0xffffffffu, me);
-        found = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
-      } else {
-        left -= whole;
-      }
+      const unsigned front = upto - __popc(mine8);
+      const bool me = left >= front && left < upto;
+      const int at = me ? s.first + (i0 + eighth * 32 + lane) * Share<T>::kPer + nth_bit(mine8, left - front) : 0;
+      const unsigned who = __ballot_sync(0xffffffffu, me);
+      found = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
     }
     if (found < 0) found = s.tail0 + nth_bit(mt, left);
   }
   if (lane == 0) a.tokens[r] = found;
+}
+
+// Writes the row's outcome: the index of the nth (from 0) of `ties` elements that equal `value`, and the log-probability
+// (value - top) / T - log(kept), with per = log2(e) / T. The first is a minimum over the cluster; of a few, the indices are
+// collected in rank 0's `list` (kTies places) and each looks how many stand in front of it.
+constexpr unsigned kTies = 1024;
+template <typename T>
+__device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args& a, int r, int c, int rank, float value, unsigned nth, unsigned ties,
+                                      unsigned* list, float top, double per, double kept, const double* table) {
+  const auto outcome = [&]() {
+    // log(kept) = y + log(kept e^-y) with y the logarithm in 32 bits: the second one is its argument less 1
+    const double y = logf(static_cast<float>(kept));
+    const double fine = kept * two_to_minus(y * 1.4426950408889634, table) - 1.0;
+    const double distance = value == top ? 0.0 : (static_cast<double>(top) - static_cast<double>(value)) * per * 0.69314718055994530942;
+    a.logprobs[r] = static_cast<float>(-distance - (y + fine));
+  };
+  if (nth > 0 && ties > kTies) {
+    if (rank == 0 && threadIdx.x == kThreads - 1) outcome();
+    place_among_many(s, sh, a, r, c, rank, value, nth);
+    return;
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  unsigned* const lead_n = c > 1 ? cl.map_shared_rank(&sh.found_n, 0) : &sh.found_n;
+  unsigned* const lead_min = c > 1 ? cl.map_shared_rank(&sh.found_min, 0) : &sh.found_min;
+  unsigned* const lead_list = c > 1 ? cl.map_shared_rank(list, 0) : list;
+  unsigned least = 0xffffffffu;
+  const auto hit = [&](unsigned at) {
+    if (nth == 0) least = min(least, at);
+    else lead_list[atomicAdd(lead_n, 1u)] = at;
+  };
+  if (static_cast<int>(threadIdx.x) < s.head && value_of<T>(s.row[threadIdx.x]) == value) hit(threadIdx.x);
+  if (s.tail0 + static_cast<int>(threadIdx.x) < s.tail1 && value_of<T>(s.row[s.tail0 + threadIdx.x]) == value) hit(s.tail0 + threadIdx.x);
+  const auto look = [&](const uint4& w, int i) {
+    for (unsigned m = s.equal(w, value); m; m &= m - 1) hit(s.first + i * Share<T>::kPer + __ffs(m) - 1);
+  };
+  int i = s.lo + threadIdx.x;
+  if (s.cached) {
+    for (; i < s.hi; i += kThreads) look(kept_pieces[i - s.lo], i);
+  } else {
+    for (; i + 3 * kThreads < s.hi; i += 4 * kThreads) {
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = s.vec[i + q * kThreads];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) look(w[q], i + q * kThreads);
+    }
+    for (; i < s.hi; i += kThreads) look(s.vec[i], i);
+  }
+  if (nth == 0) {
+    least = warp_all(least, [](unsigned x, unsigned y) { return min(x, y); });
+    if ((threadIdx.x & 31) == 0 && least != 0xffffffffu) atomicMin(lead_min, least);
+  }
+  if (c > 1) cl.sync();               // the last time that anybody reaches into a peer
+  else __syncthreads();
+  if (rank != 0) return;
+  if (threadIdx.x == kThreads - 1) outcome();
+  if (nth == 0) {
+    if (threadIdx.x == 0) a.tokens[r] = sh.found_min;
+    return;
+  }
+  for (unsigned t = threadIdx.x; t < ties; t += kThreads) {
+    const unsigned at = list[t];
+    unsigned front = 0;
+    for (unsigned j = 0; j < ties; ++j) front += list[j] < at;
+    if (front == nth) a.tokens[r] = at;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ bf16
@@ -370,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   const Row row(a, r);
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
   fill_table(table);
+  if (tid == 0) sh.found_n = 0u, sh.found_min = 0xffffffffu;
   float top, low;
   extremes(s, sh, c, top, low);
   cg::cluster_group cl = cg::this_cluster();
@@ -380,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       return;
     }
     if (rank == 0 && tid == 0) a.marked[r] = 0;
-    place(s, sh, a, r, c, rank, top, 0u, top, 1.0, 1.0);
+    place(s, sh, a, r, c, rank, top, 0u, 1u, bins, top, 1.0, 1.0, table);
     return;
   }
   low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
@@ -611,6 +690,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       for (int j = 0; j < kEach; ++j) {
         if (before >= cc && before < cc + n[j]) {
           sh.nth = before - cc;
+          sh.ties = n[j];
           sh.value = value_at(j);
           sh.state = 1;
         }
@@ -634,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     if (c > 1) cl.sync();               // peers have read this CTA's outcome
     return;
   }
-  place(s, sh, a, r, c, rank, value, nth, top, row.T, kept_mass);
+  place(s, sh, a, r, c, rank, value, nth, lead->ties, bins, top, per, kept_mass, table);
 }
 
 // ------------------------------------------------------------------------------------------------ any type
@@ -667,15 +747,21 @@ __device__ __forceinline__ u64 units_of(double t, const double* table) {
   return t < 64.0 ? static_cast<u64>(two_to_minus(t, table) * kUnit + 0.5) : 0ull;      // nothing in units of 2^-44
 }
 
+// A 64-bit sum in two words of shared memory: whoever carries the low one over adds the carry to the high one. (An atomic
+// on 64 bits there is a loop of compare and swap: 14 ns for a warp's, against 3 for these.)
+__device__ __forceinline__ void add_units(unsigned* low, unsigned* high, u64 q) {
+  const unsigned ql = static_cast<unsigned>(q), old = atomicAdd(low, ql), qh = static_cast<unsigned>(q >> 32) + (old + ql < ql ? 1u : 0u);
+  if (qh) atomicAdd(high, qh);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_constant__ Args a) {
-  __shared__ unsigned cnt[kSteps];
-  __shared__ u64 mas[kSteps];
-  __shared__ unsigned dcnt[256];
-  __shared__ u64 dmas[256];
+  __shared__ unsigned cnt[kSteps], low_half[kSteps], high_half[kSteps];       // tokens, and their weight in two words
+  __shared__ unsigned dcnt[256], dlow[256], dhigh[256];
   __shared__ Shared sh;
   __shared__ Step step[3][5];
   __shared__ unsigned list[kList], list_n;
+  __shared__ u64 list_units[kList];
   __shared__ double table[64];
   const int c = gridDim.x, rank = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   if (a.marked != nullptr) {
@@ -685,8 +771,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   cg::cluster_group cl = cg::this_cluster();
   const Share<T> s(a, r, rank, c);
   const Row row(a, r);
-  for (int i = tid; i < kSteps; i += kThreads) cnt[i] = 0u, mas[i] = 0ull;
+  for (int i = tid; i < kSteps; i += kThreads) cnt[i] = 0u, low_half[i] = 0u, high_half[i] = 0u;
   fill_table(table);
+  if (tid == 0) sh.found_n = 0u, sh.found_min = 0xffffffffu;
   float top, low;
   extremes(s, sh, c, top, low);
   if (top == -INFINITY || row.greedy) {
@@ -695,12 +782,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY;
       return;
     }
-    place(s, sh, a, r, c, rank, top, 0u, top, 1.0, 1.0);
+    place(s, sh, a, r, c, rank, top, 0u, 1u, list, top, 1.0, 1.0, table);
     return;
   }
   low = top == INFINITY ? top : fmaxf(fmaxf(low, -FLT_MAX), top - kWindow * static_cast<float>(row.T));
-  // steps of a power of two, at most kSteps of them; the quotient is rounded but grows with the distance
-  const float inv = top > low ? ldexpf(1.f, 10 - ilogbf(top - low)) : 0.f;
+  // equal steps; the product is rounded but never falls as the distance grows
+  const float inv = top > low ? static_cast<float>(kSteps) / (top - low) : 0.f;
   const auto bin_of = [&](float x) {
     const float q = (top - x) * inv;
     return q < static_cast<float>(kSteps - 1) ? static_cast<int>(q) : q >= static_cast<float>(kSteps - 1) ? kSteps - 1 : 0;
@@ -714,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     const u64 q = units(x);
     const int b = bin_of(x);
     atomicAdd(&cnt[b], 1u);
-    atomicAdd(&mas[b], q);
+    add_units(&low_half[b], &high_half[b], q);
     // on the border itself (a unit is 2^-44) the weight decides
     if (row.min_p > 0.0) some += fabs(static_cast<double>(q) - floor_units) > 2.0 ? static_cast<double>(q) > floor_units : weight(x, top, row.T) >= row.min_p;
     else ++some;
@@ -730,17 +817,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   cl.sync();
   if (c > 1) {                                         // each CTA adds up its share of the steps and puts it into rank 0's
     unsigned* lead_cnt = cl.map_shared_rank(cnt, 0);
-    u64* lead_mas = cl.map_shared_rank(mas, 0);
+    unsigned* lead_low = cl.map_shared_rank(low_half, 0);
+    unsigned* lead_high = cl.map_shared_rank(high_half, 0);
     for (int i = kSteps / c * rank + tid; i < kSteps / c * (rank + 1); i += kThreads) {
-      unsigned v[kMaxCluster], x = 0;
-      u64 w[kMaxCluster], y = 0;
+      unsigned v[kMaxCluster], l[kMaxCluster], h[kMaxCluster], x = 0;
+      u64 y = 0;
 #pragma unroll
       for (int q = 0; q < kMaxCluster; ++q)
-        if (q < c) v[q] = *cl.map_shared_rank(cnt + i, q), w[q] = *cl.map_shared_rank(mas + i, q);
+        if (q < c) v[q] = *cl.map_shared_rank(cnt + i, q), l[q] = *cl.map_shared_rank(low_half + i, q), h[q] = *cl.map_shared_rank(high_half + i, q);
 #pragma unroll
       for (int q = 0; q < kMaxCluster; ++q)
-        if (q < c) x += v[q], y += w[q];
-      lead_cnt[i] = x, lead_mas[i] = y;
+        if (q < c) x += v[q], y += (static_cast<u64>(h[q]) << 32) + l[q];
+      lead_cnt[i] = x, lead_low[i] = static_cast<unsigned>(y), lead_high[i] = static_cast<unsigned>(y >> 32);
     }
     cl.sync();
   }
@@ -751,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   if (rank == 0) {
 #pragma unroll
     for (int j = 0; j < kStepsEach; ++j) {
-      n[j] = cnt[tid * kStepsEach + j], m[j] = mas[tid * kStepsEach + j];
+      n[j] = cnt[tid * kStepsEach + j], m[j] = (static_cast<u64>(high_half[tid * kStepsEach + j]) << 32) + low_half[tid * kStepsEach + j];
       count += n[j], mass += m[j];
     }
     unsigned fine = 0;
@@ -807,14 +895,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       cl.sync();
       if (rank == 0) {
         const unsigned many = list_n;
+        for (unsigned i = tid; i < many; i += kThreads) list_units[i] = units(key_value(list[i]));
+        __syncthreads();
         for (unsigned i = tid; i < many; i += kThreads) {
           const unsigned k = list[i];
           unsigned dc = seen, dn = 0u;
           u64 dw = weighed;
-          const u64 q = units(key_value(k));
+          const u64 q = list_units[i];
+#pragma unroll 4
           for (unsigned j = 0; j < many; ++j) {
             const unsigned o = list[j];
-            if (o > k) ++dc, dw += units(key_value(o));
+            const u64 oq = list_units[j];
+            if (o > k) ++dc, dw += oq;
             dn += o == k;
           }
           if (here(what, dc, dn, dw, dw + dn * q, aim, what == 2 ? last : keep)) sh.i0 = k, sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
@@ -825,14 +917,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     }
     for (int level = 0; level < 4 && !first.few; ++level) {
       const int shift = 24 - 8 * level;
-      if (tid < 256) dcnt[tid] = 0u, dmas[tid] = 0ull;
+      if (tid < 256) dcnt[tid] = 0u, dlow[tid] = 0u, dhigh[tid] = 0u;
       __syncthreads();
       s.each([&](float x) {
         if (!(x >= low) || bin_of(x) != first.bin) return;
         const unsigned k = order_key(x);
         if (level > 0 && (k >> (shift + 8)) != prefix) return;
         atomicAdd(&dcnt[(k >> shift) & 255u], 1u);
-        atomicAdd(&dmas[(k >> shift) & 255u], units(x));
+        add_units(&dlow[(k >> shift) & 255u], &dhigh[(k >> shift) & 255u], units(x));
       });
       cl.sync();
       if (rank == 0) {
@@ -840,14 +932,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         unsigned dn = 0, dc = 0, da;
         u64 dm = 0, dw = 0, db;
         if (tid < 256) {
-          unsigned v[kMaxCluster];
-          u64 w[kMaxCluster];
+          unsigned v[kMaxCluster], l[kMaxCluster], h[kMaxCluster];
 #pragma unroll
           for (int q = 0; q < kMaxCluster; ++q)
-            if (q < c) v[q] = *cl.map_shared_rank(dcnt + 255 - tid, q), w[q] = *cl.map_shared_rank(dmas + 255 - tid, q);
+            if (q < c) v[q] = *cl.map_shared_rank(dcnt + 255 - tid, q), l[q] = *cl.map_shared_rank(dlow + 255 - tid, q), h[q] = *cl.map_shared_rank(dhigh + 255 - tid, q);
 #pragma unroll
           for (int q = 0; q < kMaxCluster; ++q)
-            if (q < c) dn += v[q], dm += w[q];
+            if (q < c) dn += v[q], dm += (static_cast<u64>(h[q]) << 32) + l[q];
         }
         dc = dn, dw = dm;
         block_prefix(dc, dw, sh.sc, sh.su, da, db);
@@ -880,6 +971,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         if (tid == 0) {
           sh.nth = at < 0.0 ? 0u : at < have ? static_cast<unsigned>(at) : have - 1u;
           sh.value = x;
+          sh.ties = sh.c1;
           sh.f1 = kept / kUnit;
         }
       }
@@ -891,11 +983,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   const float value = lead->value;
   const unsigned nth = lead->nth;
   const double kept_mass = lead->f1;
-  place(s, sh, a, r, c, rank, value, nth, top, row.T, kept_mass);
+  place(s, sh, a, r, c, rank, value, nth, lead->ties, list, top, per, kept_mass, table);
 }
 
 int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem, bool early, cudaStream_t s) {
-  if (smem > 16 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 4 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = smem;
   cfg.gridDim = dim3(cluster, rows);
@@ -940,7 +1032,7 @@ IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int
   int c = 1;
   while (c < kMaxCluster && rows * c * 2 <= 148 * 2 && V > c * 8192) c *= 2;
   const long long bytes = (static_cast<long long>(V) * (dtype == 0 ? 2 : 4) / c + 32 + 15) / 16 * 16;
-  a.cached = bytes <= 72 * 1024;
+  a.cached = bytes <= (static_cast<long long>(rows) * c <= 148 ? 160 : 60) * 1024;
   const int smem = a.cached ? static_cast<int>(bytes) : 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, smem, false, s);
