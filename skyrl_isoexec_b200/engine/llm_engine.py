@@ -40,6 +40,7 @@ class EngineConfig:
     share_prompt_pages: bool = True      # samples of one prompt share its full KV pages (not a cache: freed with the requests)
     share_recurrent_state: bool = False  # models with GatedDeltaNet layers: siblings also start from the leader's recurrent
                                          # state at the shared boundary (a snapshot taken when its prefill gets there)
+    sample_from_numbers: bool = False    # top-k / top-p / min-p rows drawn by one kernel from one number each (engine/sampler.py)
 
 
 @dataclass
@@ -67,6 +68,12 @@ class Sequence:
     mm_feats: torch.Tensor | None = None
     mm_key: bytes | None = None
     prompt_logprobs: list | None = None     # requested with SamplingParams.prompt_logprobs: [None, lp(token 1 | token 0), ...]
+    adapter: int = -1                       # place in the engine's adapter bank; -1: the base model
+
+    @property
+    def keyed_by_tokens(self) -> bool:
+        """Whether this sequence's pages are a function of its tokens alone (no images, no adapter): only such pages are cached."""
+        return self.mm_feats is None and self.adapter < 0
 
     @property
     def tokens(self) -> list[int]:
@@ -123,7 +130,7 @@ class Scheduler:
         return True
 
     def _preempt(self, seq: Sequence) -> None:
-        if self.prefix is not None and seq.mm_feats is None:
+        if self.prefix is not None and seq.keyed_by_tokens:
             self.prefix.insert(seq.tokens, seq.pages, seq.num_computed)  # the recompute may find them again
         self.cache.allocator.release(seq.pages)
         seq.pages = []
@@ -195,7 +202,7 @@ class Scheduler:
                     self.shared_prompt_tokens += s.shared_tokens
                     if self.adopt_hook is not None:
                         self.adopt_hook(s, ld)
-            if self.prefix is not None and s.leader is None and not s.pages and s.num_computed == 0 and s.mm_feats is None \
+            if self.prefix is not None and s.leader is None and not s.pages and s.num_computed == 0 and s.keyed_by_tokens \
                     and s.prompt_logprobs is None:
                 pages, key = self.prefix.match(s.tokens)
                 if pages:
@@ -212,7 +219,7 @@ class Scheduler:
         return decode, prefill
 
     def finish(self, seq: Sequence) -> None:
-        if self.prefix is not None and seq.mm_feats is None:      # pages are keyed by tokens alone: image prompts stay out
+        if self.prefix is not None and seq.keyed_by_tokens:       # pages are keyed by tokens alone: image prompts stay out
             self.prefix.insert(seq.tokens, seq.pages, seq.num_computed)
         self.cache.allocator.release(seq.pages)
         seq.pages = []
@@ -229,7 +236,8 @@ class LLMEngine:
         n_pages = self.cfg.num_kv_pages or self._auto_pages()
         self.cache = KVCache(self.mcfg, n_pages, self.device, tp=model.ps.tp, layer_ids=model.layer_ids)
         self.scheduler = Scheduler(self.cfg, self.cache)
-        self.sampler = Sampler(self.device, self.cfg.seed, self.mcfg.logprob_leaves)
+        self.sampler = Sampler(self.device, self.cfg.seed, self.mcfg.logprob_leaves, from_numbers=self.cfg.sample_from_numbers)
+        self.adapters = None            # AdapterBank: requests may name one of its adapters (set_adapters)
         self._next_id = 0
         self.detokenize = None          # ids -> text, set by whoever owns a tokenizer; needed only for stop STRINGS
         self.paused = False
@@ -327,7 +335,7 @@ class LLMEngine:
         still runs), and for a model with recurrent layers keep the state at a page boundary the sequence stands on
         exactly (its open chunk is empty there)."""
         pc = self.prefix_cache
-        if pc is None or s.num_computed < PAGE or not (prefill or s.num_computed % PAGE == 0) or s.mm_feats is not None:
+        if pc is None or s.num_computed < PAGE or not (prefill or s.num_computed % PAGE == 0) or not s.keyed_by_tokens:
             return
         if pc.boundary is not None:
             if s.num_computed % PAGE or s.seq_id not in self.gdn_state.row_of:
@@ -352,16 +360,34 @@ class LLMEngine:
     def resume_generation(self) -> None:
         self.paused = False
 
+    def set_adapters(self, bank) -> None:
+        """Serve the adapters of ``bank`` (``train/lora.AdapterBank``, or None for none): a request that names one computes with
+        ``W + s B A`` on the bank's targets while its neighbours in the batch use others or none. A row without an adapter keeps
+        the base model's bits; rows with one are outside the execution contract (the trainer merges its adapter into ``W``). Such
+        batches step eagerly, and their pages are not cached."""
+        if bank is not None and self.model.ps.tp * self.model.ps.pp * self.model.ps.ep * self.model.ps.cp > 1:
+            raise ValueError("adapters of many requests need tensor-, pipeline-, expert- and context-parallel degrees of 1")
+        self._drain_inflight()
+        if any(s.adapter >= 0 for s in [*self.scheduler.waiting, *self.scheduler.running]):
+            raise RuntimeError("set_adapters with requests in flight that use the present ones")
+        self.adapters = bank
+
     # ------------------------------------------------------------------ requests
-    def add_request(self, prompt_ids: list[int], params: SamplingParams, request_index: int = 0, mm: dict | None = None) -> Sequence:
-        """``mm``: ``{"pixel_values": [patches, dim], "image_grid_thw": [images, 3], "positions": optional list}`` for a
+    def add_request(self, prompt_ids: list[int], params: SamplingParams, request_index: int = 0, mm: dict | None = None,
+                    adapter: str | None = None) -> Sequence:
+        """``adapter``: the name of one of the bank's adapters (``set_adapters``). ``mm``: ``{"pixel_values": [patches, dim], "image_grid_thw": [images, 3], "positions": optional list}`` for a
         prompt with image placeholder tokens (``positions``: where they are; default: every token equal to the model's
         ``image_token_id``). The vision tower runs here, once per request."""
         if len(prompt_ids) == 0:
             raise ValueError("empty prompt")
         if len(prompt_ids) >= self.max_len:
             raise ValueError(f"prompt of {len(prompt_ids)} tokens exceeds max_model_len={self.max_len}")
-        seq = Sequence(self._next_id, list(prompt_ids), params, request_index=request_index, arrival=time.time())
+        place = -1
+        if adapter is not None:
+            if self.adapters is None or adapter not in self.adapters.names:
+                raise ValueError(f"unknown adapter {adapter!r}: the engine serves {self.adapters.names if self.adapters is not None else []}")
+            place = self.adapters.names.index(adapter)
+        seq = Sequence(self._next_id, list(prompt_ids), params, request_index=request_index, arrival=time.time(), adapter=place)
         self._next_id += 1
         if mm is not None and mm.get("pixel_values") is not None and mm["pixel_values"].shape[0]:
             self._attach_images(seq, mm)
@@ -427,15 +453,15 @@ class LLMEngine:
         decode, prefill = self.scheduler.schedule()
         if not decode and not prefill:
             return []
-        if not prefill and self._graphs_enabled() and not any(_needs_history(s.params) for s in decode):
+        if not prefill and self._graphs_enabled() and not any(_needs_history(s.params) or s.adapter >= 0 for s in decode):
             # (a request whose sampling looks at its own tokens cannot run ahead of the host: the token in flight is part
-            # of that history)
+            # of that history; the captured step computes with the base weights alone)
             self._inflight = self._launch_decode(decode, ahead=False)
             return []
         G = self.model.hq // self.model.hkv
         tq = PAGE // G
         ids, pos, slots, items, bt_rows, sample_rows, sample_seqs = [], [], [], [], [], [], []
-        mm_rows, mm_feats = [], []
+        mm_rows, mm_feats, adapter_of = [], [], []
         row = 0
         for s in decode:
             p = s.length - 1
@@ -446,6 +472,7 @@ class LLMEngine:
             bt_rows.append(s.pages)
             sample_rows.append(row)
             sample_seqs.append(s)
+            adapter_of.append(s.adapter)
             row += 1
         for s, start, n in prefill:
             toks = s.tokens
@@ -464,6 +491,7 @@ class LLMEngine:
                 if r:
                     mm_rows += r
                     mm_feats.append(f)
+            adapter_of += [s.adapter] * n
             row += n
         maxp = max(len(b) for b in bt_rows)
         bt = torch.zeros(len(bt_rows), maxp, dtype=torch.int32)
@@ -481,6 +509,8 @@ class LLMEngine:
             fc.kv = self.gdn_state.merge_into(self.cache.pools)
         if mm_rows:
             fc.mm = (self._h2d(torch.tensor(mm_rows, dtype=torch.int64)), torch.cat(mm_feats, 0))
+        if any(a >= 0 for a in adapter_of):
+            fc.lora = self.adapters.batch(self._h2d(torch.tensor(adapter_of, dtype=torch.int32)))
         hidden = self.model(self._h2d(torch.tensor(ids, dtype=torch.int64)), fc)
         if any(s.prompt_logprobs is not None for s, _, _ in prefill):
             self._fill_prompt_logprobs(hidden, prefill, len(decode))
@@ -706,7 +736,7 @@ class LLMEngine:
                 continue                                        # already under way
             if s.prompt_logprobs is not None:
                 continue                                        # every prompt row of such a request must be computed
-            ld = leaders.setdefault((tuple(s.prompt_ids), s.mm_key), s)
+            ld = leaders.setdefault((tuple(s.prompt_ids), s.mm_key, s.adapter), s)
             shared = ((len(s.prompt_ids) - 1) // PAGE) * PAGE   # a multiple of the GatedDeltaNet chunk too: no open chunk there
             if ld is not s and shared > 0:
                 s.leader, s.shared_tokens = ld, shared
@@ -715,14 +745,18 @@ class LLMEngine:
                 n += 1
         return n
 
-    def generate(self, prompts: list[list[int]], params: SamplingParams | list[SamplingParams], mm: list | None = None) -> list[RequestOutput]:
+    def generate(self, prompts: list[list[int]], params: SamplingParams | list[SamplingParams], mm: list | None = None,
+                 adapters: list | None = None) -> list[RequestOutput]:
         """Blocking batch generation; outputs are in prompt order. ``mm``: per prompt, the image inputs of ``add_request``
-        or None."""
+        or None. ``adapters``: per prompt, the name of its adapter or None."""
         if self.asleep:
             raise RuntimeError("engine is asleep; call wake_up() first")
         plist = params if isinstance(params, list) else [params] * len(prompts)
         mlist = mm if mm is not None else [None] * len(prompts)
-        seqs = [self.add_request(p, sp, i, mm=m) for i, (p, sp, m) in enumerate(zip(prompts, plist, mlist))]
+        alist = adapters if adapters is not None else [None] * len(prompts)
+        if len(alist) != len(prompts):
+            raise ValueError(f"{len(alist)} adapters for {len(prompts)} prompts")
+        seqs = [self.add_request(p, sp, i, mm=m, adapter=ad) for i, (p, sp, m, ad) in enumerate(zip(prompts, plist, mlist, alist))]
         self.link_samples(seqs)
         while True:
             if self.paused:

@@ -6,6 +6,11 @@ ISO/runtimes/vllm/vllm_patches.py:388), computed by the same fixed-leaf kernel t
 scores with (ops/functional.token_logprobs). Temperature / top-k / top-p / min-p only shape
 the distribution the token is drawn from; drawing uses the Gumbel-max trick so one
 generator seed fixes the whole rollout.
+
+With ``from_numbers`` the truncated requests are drawn by ``ops/sampling.sample_rows`` instead of row by row: one uniform number
+per row from the same generator, one kernel for the whole batch, whatever its requests' settings. The distribution is the same
+but for ties (``top_k`` keeps exactly k tokens, the lowest indices among equal logits, where the row-by-row form keeps all that
+equal the k-th); the numbers are consumed differently, so a seed gives other tokens than without it.
 """
 
 from __future__ import annotations
@@ -72,8 +77,9 @@ def isoexec_sampling_constraints(p: SamplingParams) -> SamplingParams:
 
 
 class Sampler:
-    def __init__(self, device, seed: int = 0, leaves: int = F.DEFAULT_LEAVES):
+    def __init__(self, device, seed: int = 0, leaves: int = F.DEFAULT_LEAVES, from_numbers: bool = False):
         self.device = torch.device(device)
+        self.from_numbers = from_numbers
         self.gen = torch.Generator(device=self.device)
         self.gen.manual_seed(seed)
         self.leaves = leaves
@@ -114,6 +120,25 @@ class Sampler:
         logprobs, _ = F.token_logprobs(logits, tokens, self.leaves)
         return tokens, logprobs
 
+    def _by_numbers(self, x: torch.Tensor, params: list[SamplingParams]) -> torch.Tensor:
+        """Tokens of rows with settings of their own, one uniform number each (``ops/sampling.sample_rows``)."""
+        from ..ops.sampling import sample_rows
+
+        n, p0 = x.shape[0], params[0]
+        same = all(p is p0 for p in params)
+        each = lambda p: (p.temperature, p.top_k, p.top_p, p.min_p)  # noqa: E731
+        key = ("rows", each(p0), n) if same else ("rows", tuple(each(p) for p in params))
+        settings = self._temp_cache.get(key)
+        if settings is None:
+            if len(self._temp_cache) > 64:
+                self._temp_cache.clear()
+            cols = list(zip(*([each(p0)] * n if same else [each(p) for p in params])))
+            f32 = lambda v: torch.tensor(v, dtype=torch.float32).to(x.device)  # noqa: E731
+            k = torch.tensor([v if v and v > 0 else 0 for v in cols[1]], dtype=torch.int64).clamp(max=2 ** 31 - 1).to(torch.int32).to(x.device)
+            settings = self._temp_cache[key] = (f32(cols[0]), k, f32(cols[2]), f32(cols[3]))
+        u = torch.rand(n, device=x.device, dtype=torch.float32, generator=self.gen)
+        return sample_rows(x, u, *settings)[0]
+
     @staticmethod
     def _shape_row(row: torch.Tensor, p: SamplingParams, history, eos_token_id) -> torch.Tensor:
         """Penalties, bias and the ``min_tokens`` mask on one row of fp32 logits (before the temperature, as vLLM does)."""
@@ -151,6 +176,16 @@ class Sampler:
         untruncated = all(p.top_p >= 1.0 and p.top_k <= 0 and p.min_p <= 0.0 for p in params) and not any(shaped)
         if untruncated and logits.is_cuda and logits.dtype == torch.bfloat16 and logits.stride(1) == 1 and logits.stride(0) % 8 == 0:
             return self._fused(logits, params)
+        if self.from_numbers:
+            x = logits
+            if any(shaped):
+                x = logits.float()
+                x = x.clone() if x is logits else x
+                for i, p in enumerate(params):
+                    if shaped[i]:
+                        x[i] = self._shape_row(x[i], p, histories[i] if histories is not None else None, eos_token_id)
+            tokens = self._by_numbers(x if x.dtype in (torch.bfloat16, torch.float32) else x.float(), params)
+            return tokens, F.token_logprobs(logits, tokens, self.leaves)[0]
         x = logits.float()
         uniform = all(p.temperature == 1.0 and p.top_p >= 1.0 and p.top_k <= 0 and p.min_p <= 0.0 for p in params) and not any(shaped)
         if not uniform:

@@ -242,6 +242,7 @@ class ForwardCtx:
     site: str = "trainer_fwd"          # trainer_fwd | trainer_score | engine_prefill | engine_decode
     sp_T: int | None = None            # set by the forward when sequence parallelism is on: total rows of the micro-batch
     mm: tuple | None = None            # vision-language: (rows int64 [n], features [n, hidden]) that replace embedding rows
+    lora: object | None = None         # adapters of this batch's tokens (train/lora.py::LoraBatch); tp = cp = 1
 
 
 class DecoderLM(nn.Module):
@@ -302,11 +303,21 @@ class DecoderLM(nn.Module):
             return w
         return self.p("lm_head.weight")
 
+    def _proj(self, x: torch.Tensor, name: str, fc: ForwardCtx | None) -> torch.Tensor:
+        """The projection ``name`` of x, with the adapters of the batch's tokens beside it where they have one."""
+        lora = fc.lora if fc is not None else None
+        return lora.linear(x, self.p(name), name) if lora is not None and name in lora else F.linear(x, self.p(name))
+
+    def _beside(self, y: torch.Tensor, x: torch.Tensor, name: str, fc: ForwardCtx | None) -> torch.Tensor:
+        """y = the row-parallel projection ``name`` of x, plus the adapters of the batch's tokens."""
+        lora = fc.lora if fc is not None else None
+        return lora.add(y, x, name) if lora is not None and name in lora else y
+
     # -------------------------------------------------------------------------------- layers
     def _attn_block(self, i: int, y: torch.Tensor, fc: ForwardCtx, kv_idx: int) -> torch.Tensor:
         cfg, pfx = self.cfg, f"layers.{i}.attn."
         T = fc.sp_T if fc.sp_T is not None else y.shape[0]
-        qkv = F.linear(tp_ops.copy_to_tp(y, self.ps, fc.sp_T), self.p(pfx + "qkv.weight"))
+        qkv = self._proj(tp_ops.copy_to_tp(y, self.ps, fc.sp_T), pfx + "qkv.weight", fc)
         qw = self.p(pfx + "q_norm.weight") if cfg.qk_norm else None
         kw = self.p(pfx + "k_norm.weight") if cfg.qk_norm else None
         if fc.kv is None:
@@ -327,8 +338,8 @@ class DecoderLM(nn.Module):
             a, _ = F.attention_fwd(q, k_pool, v_pool, fc.meta, self.scale)
         if cfg.attn_output_gate:
             a = _gate_attn(a, qkv, self.hq, self.hkv, cfg.head_dim)
-        return tp_ops.row_parallel_linear(a.reshape(T, self.hq * cfg.head_dim), self.p(pfx + "o.weight"), self.ps, cfg,
-                                          sp=fc.sp_T is not None)
+        a = a.reshape(T, self.hq * cfg.head_dim)
+        return self._beside(tp_ops.row_parallel_linear(a, self.p(pfx + "o.weight"), self.ps, cfg, sp=fc.sp_T is not None), a, pfx + "o.weight", fc)
 
     def _mla_block(self, i: int, y: torch.Tensor, fc: ForwardCtx, kv_idx: int) -> torch.Tensor:
         """Multi-head latent attention (reference model: R/tx/models/deepseekv3.py) in its materialised form: the latent
@@ -342,11 +353,11 @@ class DecoderLM(nn.Module):
             qa, _ = F.rmsnorm(F.linear(y, self.p(pfx + "q_a.weight")), self.p(pfx + "q_a_norm.weight"), cfg.rms_eps, False)
         else:
             qa = y
-        q = F.linear(tp_ops.copy_to_tp(qa, ps), self.p(pfx + "q_b.weight")).view(T, H, D)
+        q = self._proj(tp_ops.copy_to_tp(qa, ps), pfx + "q_b.weight", fc).view(T, H, D)
         kva = F.linear(y, self.p(pfx + "kv_a.weight"))
         c, _ = F.rmsnorm(kva[:, :r].contiguous(), self.p(pfx + "kv_a_norm.weight"), cfg.rms_eps, False)
         k_rot = tp_ops.copy_to_tp(kva[:, r:].contiguous(), ps)                  # one rotated key shared by all heads
-        kvb = F.linear(tp_ops.copy_to_tp(c, ps), self.p(pfx + "kv_b.weight")).view(T, H, dn + dv)
+        kvb = self._proj(tp_ops.copy_to_tp(c, ps), pfx + "kv_b.weight", fc).view(T, H, dn + dv)
         k = torch.cat([k_rot.unsqueeze(1).expand(T, H, dr), kvb[..., :dn]], dim=-1)
         v = kvb[..., dn:]
         if dv < D:
@@ -361,7 +372,7 @@ class DecoderLM(nn.Module):
                                    False, False, False)
             a, _ = F.attention_fwd(q, k_pool, v_pool, fc.meta, self.scale)
         a = a[..., :dv].reshape(T, H * dv) if dv < D else a.reshape(T, H * D)
-        return tp_ops.row_parallel_linear(a, self.p(pfx + "o.weight"), ps, cfg)
+        return self._beside(tp_ops.row_parallel_linear(a, self.p(pfx + "o.weight"), ps, cfg), a, pfx + "o.weight", fc)
 
     def _mlp_block(self, i: int, y: torch.Tensor, fc: ForwardCtx | None = None) -> torch.Tensor:
         cfg, pfx = self.cfg, f"layers.{i}."
@@ -371,15 +382,17 @@ class DecoderLM(nn.Module):
         sp_T = fc.sp_T if fc is not None else None
         if sp_T is not None:
             y = tp_ops.copy_to_tp(y, self.ps, sp_T)              # all rows for the column-parallel gate|up GEMM
-        if y.is_cuda and y.dtype == torch.bfloat16 and not torch.is_grad_enabled() and (wgu.shape[0] // 2) % 32 == 0 and y.dim() == 2:
+        lora = fc.lora if fc is not None else None
+        apart = lora is not None and pfx + "mlp.gate_up.weight" in lora          # an adapter is added in front of the activation
+        if y.is_cuda and y.dtype == torch.bfloat16 and not torch.is_grad_enabled() and (wgu.shape[0] // 2) % 32 == 0 and y.dim() == 2 and not apart:
             # gate_up GEMM with the SwiGLU applied in its epilogue (one launch, no [T, 2F] intermediate). The epilogue
             # repeats the roundings of the separate kernels, so this and the differentiable path below agree bit for bit.
             _obs.note("mm", "tcgen05_batch_invariant")
             _obs.note("activation.swiglu", "fused_swiglu")
             a = moe_ops.grouped_gemm(y, wgu.unsqueeze(0), None, moe_ops.EPI_GLU)
         else:
-            a = F.swiglu(F.linear(y if sp_T is not None else tp_ops.copy_to_tp(y, self.ps), wgu))
-        return tp_ops.row_parallel_linear(a, self.p(pfx + "mlp.down.weight"), self.ps, cfg, sp=sp_T is not None)
+            a = F.swiglu(self._proj(y if sp_T is not None else tp_ops.copy_to_tp(y, self.ps), pfx + "mlp.gate_up.weight", fc))
+        return self._beside(tp_ops.row_parallel_linear(a, self.p(pfx + "mlp.down.weight"), self.ps, cfg, sp=sp_T is not None), a, pfx + "mlp.down.weight", fc)
 
     def layer(self, i: int, x: torch.Tensor, res: torch.Tensor | None, fc: ForwardCtx, kv_idx: int):
         cfg = self.cfg
@@ -400,6 +413,8 @@ class DecoderLM(nn.Module):
         else:
             x, res = hidden_in
         fc.sp_T = None
+        if fc.lora is not None and self.ps.tp * self.ps.cp > 1:
+            raise ValueError("adapters of a batch's tokens (ForwardCtx.lora) need tensor- and context-parallel degrees of 1")
         if self._sequence_parallel(fc, hidden_in):
             # Megatron-style sequence parallelism (trainer sites): from here to the final norm every rank carries its
             # T / tp rows of the residual stream; the tensor-parallel regions gather rows on entry and keep this rank's

@@ -139,8 +139,7 @@ class SkyRLTrainBackend:
             t = self.tenants[tenant]
             lr = (req.get("adam_params") or {}).get("learning_rate")
             if lr is not None:
-                for gparam in t["trainer"].opt.param_groups:
-                    gparam["lr"] = float(lr)
+                t["trainer"].set_lr(lr)
             self.worker.reduce_gradients()
             gn = t["trainer"].optim_step()
             t["step"] += 1

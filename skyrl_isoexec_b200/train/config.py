@@ -54,6 +54,7 @@ class LoRASettings:
     lr: float = 0.0                     # 0 = the policy optimizer's learning rate
     target_modules: str = "all-linear"  # "all-linear" or a comma-separated list of parameter-name suffixes (e.g. "attn.qkv.weight")
     seed: int = 0
+    optimizer: str = "adam"             # adam | fused | fused8 (train/lora.py): the step over all factors in one launch, moments in 32 or 8 bits
 
 
 @dataclass
@@ -126,6 +127,7 @@ class InferenceEngineConfig:
                                         # when its layout is the trainer's: what lets generation run WHILE the trainer updates
     share_prompt_pages: bool = True     # the n samples of a prompt read one copy of its full KV pages (same bits; not a cache)
     share_recurrent_state: bool = False # GatedDeltaNet models: the samples also start from one snapshot of the recurrent state
+    sample_from_numbers: bool = False   # top-k / top-p / min-p rows drawn by one kernel, one random number a row (engine/sampler.py)
     weight_sync_backend: str = "nccl"   # nccl | gloo | cuda_ipc | shared
     run_engines_locally: bool = True
     enable_http_endpoint: bool = False  # the in-process engine also answers HTTP (OpenAI-style and token-level routes of engine/server.py) and

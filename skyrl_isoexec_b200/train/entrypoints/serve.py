@@ -35,6 +35,8 @@ def build(argv=None) -> InferenceServer:
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--enable-prefix-caching", action="store_true",
                     help="keep full KV pages after their request and reuse them for later requests with the same leading tokens")
+    ap.add_argument("--sample-from-numbers", action="store_true",
+                    help="draw top-k / top-p / min-p requests with one kernel for the batch, one random number a row")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     a = ap.parse_args(argv)
     model = DecoderLM(get_config(a.model), device=a.device, seed=a.seed)
@@ -47,7 +49,8 @@ def build(argv=None) -> InferenceServer:
             from ...sync.strategies import load_weights
 
             load_weights(model, torch.load(a.weights, map_location="cpu", weights_only=False)["model"].items())
-    kw = {"max_num_seqs": a.max_num_seqs, "seed": a.seed, "enable_prefix_caching": a.enable_prefix_caching}
+    kw = {"max_num_seqs": a.max_num_seqs, "seed": a.seed, "enable_prefix_caching": a.enable_prefix_caching,
+          "sample_from_numbers": a.sample_from_numbers}
     if a.num_kv_pages:
         kw["num_kv_pages"] = a.num_kv_pages
     eng = LLMEngine(model, EngineConfig(**kw))

@@ -6,6 +6,11 @@ The model computes with ONE weight buffer (shared with the colocated engine), so
 engine needs no LoRA-aware kernel and rollouts under an adapter stay bitwise equal to the trainer's scoring.
 Training an adapter: the base weights are frozen; the dense weight gradient dW that the backward already
 produces is projected onto the factors, dA = (alpha/r) * B^T dW, dB = (alpha/r) * dW A^T, and only A, B step.
+
+Several adapters at once: an ``AdapterBank`` holds their factors side by side, and a batch whose tokens use different ones
+(``ForwardCtx.lora = bank.batch(...)``, ``LLMEngine.set_adapters``) adds each token's own beside the shared projections with
+``ops/lora.py``, in serving and, differentiably, in training: one forward and backward over the sequences of many tenants, no
+dense weight gradient.
 """
 
 from __future__ import annotations
@@ -25,6 +30,7 @@ class LoRAConfig:
     targets: tuple = DEFAULT_TARGETS
     lr: float = 1e-4
     seed: int = 0
+    optimizer: str = "adam"     # "adam": torch's; "fused" / "fused8": ops/optim.TensorAdamW, one launch for all factors, moments in 32 or 8 bits
 
 
 @dataclass
@@ -120,6 +126,86 @@ class AdapterStore:
             self.activate(t)
 
 
+class AdapterBank:
+    """The factors of several adapters side by side, per target weight ``A [E, r, in]`` and ``B [E, out, r]`` in the model's type:
+    ``r`` is the largest rank, rounded up to a multiple of 8, smaller adapters are filled up with zeros, and an adapter without
+    a target has zeros there. ``trainable``: the factors take gradients (``parameters()``)."""
+
+    def __init__(self, model, adapters: dict[str, LoRAAdapter], trainable: bool = False):
+        if not adapters:
+            raise ValueError("AdapterBank: no adapters")
+        views = dict(model.named_weights())
+        self.names = list(adapters)
+        self.cfgs = [ad.cfg for ad in adapters.values()]
+        self.rank = max(-(-c.rank // 8) * 8 for c in self.cfgs)
+        dev = model.store.flat.device
+        self.scale = torch.tensor([ad.scale for ad in adapters.values()], dtype=torch.float32, device=dev)
+        self.A: dict[str, torch.Tensor] = {}
+        self.B: dict[str, torch.Tensor] = {}
+        for t in [n for n in views if any(n in ad.A for ad in adapters.values())]:
+            out, inn = views[t].shape
+            self.A[t] = torch.zeros(len(adapters), self.rank, inn, dtype=views[t].dtype, device=dev)
+            self.B[t] = torch.zeros(len(adapters), out, self.rank, dtype=views[t].dtype, device=dev)
+        for name, ad in adapters.items():
+            missing = [t for t in ad.A if t not in self.A]
+            if missing:
+                raise ValueError(f"AdapterBank: the model has no weight {missing[0]!r} that adapter {name!r} was made for")
+            self.put(name, ad)
+        for t in self.parameters():
+            t.requires_grad_(trainable)
+
+    @torch.no_grad()
+    def put(self, name: str, ad: LoRAAdapter) -> None:
+        """Take the factors of ``ad`` again (after it stepped on its own) in the place of adapter ``name``."""
+        e, r = self.names.index(name), ad.cfg.rank
+        if r > self.rank or ad.scale != float(self.scale[e]):
+            raise ValueError(f"AdapterBank: {name!r} changed its rank or scale; build a new bank")
+        for t in self.A:
+            self.A[t][e].zero_()
+            self.B[t][e].zero_()
+            if t in ad.A:
+                self.A[t][e, :r].copy_(ad.A[t])
+                self.B[t][e, :, :r].copy_(ad.B[t])
+
+    def adapter(self, name: str) -> LoRAAdapter:
+        """The factors of one adapter, in fp32 and at its own rank."""
+        e = self.names.index(name)
+        r = self.cfgs[e].rank
+        ad = LoRAAdapter(self.cfgs[e])
+        for t in self.A:
+            if t.endswith(tuple(ad.cfg.targets)):
+                ad.A[t], ad.B[t] = self.A[t][e, :r].detach().float().clone(), self.B[t][e, :, :r].detach().float().contiguous().clone()
+        return ad
+
+    def parameters(self) -> list[torch.Tensor]:
+        return [t for pair in zip(self.A.values(), self.B.values()) for t in pair]
+
+    def batch(self, ids) -> "LoraBatch":
+        """The adapters of a batch's tokens for ``ForwardCtx.lora``. ``ids``: a device tensor of places (negative: none), or a
+        list of names and None, one per token."""
+        if not isinstance(ids, torch.Tensor):
+            ids = torch.tensor([-1 if n is None else self.names.index(n) for n in ids], dtype=torch.int32, device=self.scale.device)
+        return LoraBatch(self, ids)
+
+
+class LoraBatch:
+    """One batch's tokens grouped by adapter (``ops/lora.LoraPlan``, built once) with the bank they compute with."""
+
+    def __init__(self, bank: AdapterBank, ids: torch.Tensor):
+        from ..ops import lora as ops
+
+        self._ops, self.bank, self.plan = ops, bank, ops.LoraPlan(ids, len(bank.names))
+
+    def __contains__(self, target: str) -> bool:
+        return target in self.bank.A
+
+    def linear(self, x, w, target: str):
+        return self._ops.lora_linear(x, w, self.bank.A[target], self.bank.B[target], self.bank.scale, self.plan)
+
+    def add(self, y, x, target: str):
+        return self._ops.lora_add(y, x, self.bank.A[target], self.bank.B[target], self.bank.scale, self.plan)
+
+
 class LoRATrainer:
     """Adam on the factors of one adapter, fed by the dense main gradients of a ``PolicyWorker``."""
 
@@ -131,7 +217,23 @@ class LoRATrainer:
             self.ad.A[name].requires_grad_(False)
             self.ad.B[name].requires_grad_(False)
             params += [self.ad.A[name], self.ad.B[name]]
-        self.opt = torch.optim.Adam(params, lr=self.ad.cfg.lr)
+        if self.ad.cfg.optimizer == "adam":
+            self.opt = torch.optim.Adam(params, lr=self.ad.cfg.lr)
+        elif self.ad.cfg.optimizer in ("fused", "fused8"):
+            from ..ops.optim import TensorAdamW
+
+            self.opt = TensorAdamW(params, lr=self.ad.cfg.lr, state_bits=8 if self.ad.cfg.optimizer == "fused8" else 32)
+            for p, g in zip(params, self.opt.grads):
+                p.grad = g
+        else:
+            raise ValueError(f"LoRAConfig.optimizer is 'adam', 'fused' or 'fused8', not {self.ad.cfg.optimizer!r}")
+
+    def set_lr(self, lr: float) -> None:
+        if isinstance(self.opt, torch.optim.Optimizer):
+            for group in self.opt.param_groups:
+                group["lr"] = float(lr)
+        else:
+            self.opt.lr = float(lr)
 
     @torch.no_grad()
     def optim_step(self) -> float:
@@ -145,8 +247,12 @@ class LoRATrainer:
                 n *= d
             dW = opt.main_grad[s.offset:s.offset + n].view(s.shape).float()
             A, B = self.ad.A[name], self.ad.B[name]
-            A.grad = self.ad.scale * (B.t() @ dW)
-            B.grad = self.ad.scale * (dW @ A.t())
+            if isinstance(self.opt, torch.optim.Optimizer):
+                A.grad = self.ad.scale * (B.t() @ dW)
+                B.grad = self.ad.scale * (dW @ A.t())
+            else:                                  # into the optimizer's own buffers
+                torch.mul(B.t() @ dW, self.ad.scale, out=A.grad)
+                torch.mul(dW @ A.t(), self.ad.scale, out=B.grad)
             sq += float(A.grad.square().sum() + B.grad.square().sum())
         self.opt.step()
         opt.zero_grad()

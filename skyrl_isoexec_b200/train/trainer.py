@@ -307,7 +307,8 @@ class RayPPOTrainer:
             targets = DEFAULT_TARGETS if ls.target_modules in ("all-linear", "", "all") else tuple(x.strip() for x in ls.target_modules.split(",") if x.strip())
             self.lora_store = AdapterStore(model)
             self.lora_store.register("policy", LoRAAdapter.init(model, LoRAConfig(rank=ls.rank, alpha=ls.alpha, targets=targets,
-                                                                                  lr=ls.lr or t.policy.optimizer_config.lr, seed=ls.seed)))
+                                                                                  lr=ls.lr or t.policy.optimizer_config.lr, seed=ls.seed,
+                                                                                  optimizer=ls.optimizer)))
             self.lora_store.activate("policy")
             self.policy.lora = LoRATrainer(self.policy, self.lora_store, "policy")
         if algo.use_kl_loss or algo.use_kl_in_reward:
@@ -349,7 +350,7 @@ class RayPPOTrainer:
                             num_kv_pages=ie.num_kv_pages, gpu_memory_utilization=ie.gpu_memory_utilization,
                             # one sampler stream per engine; the ranks of one engine share it
                             seed=t.seed + 7919 * self._engine_index(),
-                            enable_prefix_caching=ie.enable_prefix_caching,
+                            enable_prefix_caching=ie.enable_prefix_caching, sample_from_numbers=ie.sample_from_numbers,
                             use_cuda_graph=not ie.enforce_eager, share_prompt_pages=ie.share_prompt_pages, share_recurrent_state=ie.share_recurrent_state,
                             # a multi-turn context grows to generator.max_input_length before its last turn
                             max_model_len=min(mcfg.max_position, (max(t.max_prompt_length, g.max_input_length) if (g.max_turns > 1 or not g.batched)
