@@ -106,6 +106,15 @@ __device__ __forceinline__ void decode8(const void* codes, long long at, float s
   }
 }
 
+// Square root: the approximation and one step of Newton's method, s + (v - s^2) / (2 s), to the last place. Where v is next to
+// the smallest numbers the approximation stands (v - s^2 would be rounded away).
+__device__ __forceinline__ float root_of(float v) {
+  float s, r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return v > 1e-30f && v < 1e38f ? fmaf(fmaf(-s, s, v), 0.5f * r, s) : s;
+}
+
 // Codes and scale of the warp's 256 values. `root`: a positive value's code is at least the smallest one.
 template <bool ROOT>
 __device__ __forceinline__ void encode8(void* codes, float* scales, long long at, float (&x)[kVec]) {
@@ -135,7 +144,7 @@ __device__ __forceinline__ void encode8(void* codes, float* scales, long long at
 }
 
 template <typename P, typename G, bool BITS8>
-__global__ void __launch_bounds__(kThreads) tensor_adamw_kernel(Args a) {
+__global__ void __launch_bounds__(kThreads, BITS8 ? 5 : 4) tensor_adamw_kernel(Args a) {
   const int2 where = a.chunks[blockIdx.x];
   const Entry e = a.table[where.x];
   const long long first = static_cast<long long>(where.y) * kChunk + static_cast<long long>(threadIdx.x >> 5) * kBlock;
@@ -163,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) tensor_adamw_kernel(Args a) {
     const float vo = BITS8 ? __fmul_rn(v[j], v[j]) : v[j];
     m[j] = __fadd_rn(__fmul_rn(a.b1, m[j]), __fmul_rn(a.nb1, x));
     v[j] = __fadd_rn(__fmul_rn(a.b2, vo), __fmul_rn(__fmul_rn(a.nb2, x), x));
-    root[j] = __fsqrt_rn(v[j]);
+    root[j] = root_of(v[j]);
     p[j] = p[j] * keep - __fdividef(a.step_size * m[j], root[j] * a.rsqrt_bc2 + a.eps);
   }
   if constexpr (sizeof(P) == 2) store8(a.master + e.offset, i, e.n, true, p);
