@@ -718,10 +718,11 @@ struct GradArgs {
   const __nv_bfloat16* h;     // [2, T, r], plan's order
   const __nv_bfloat16* z;     // [T, C] rows by token
   __nv_bfloat16* out;         // [E, r, C], or by columns [E, C, r]
+  long long ld_z;
+  int C, by_cols;
   const int* perm;
   const int* offsets;
-  long long ld_z;
-  int T, C, r, by_cols;
+  int T, r;
 };
 constexpr int kTok = 64, kCols = 128, kStages = 3;
 constexpr int kZRow = kCols * 2 + 16;                  // bytes a row in shared memory: 16 more spread the transposed reads
@@ -963,33 +964,59 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   return apply_tile<16>(a, large, across, grid, s);
 }
 
-// out[a] = sum over the adapter's tokens of h[t]^T z[t]: bf16 [E, r, C], or by columns [E, C, r]; zero without tokens.
-IX_API int ix_lora_grad(const void* h, const void* z, long long ld_z, void* out, const void* perm, const void* offsets, int T, int C, int r, int E,
-                        int by_cols, void* stream) {
-  if (r < 8 || r > kMaxRank || r % 8) return ixh::fail(ixh::IX_EARG, "lora: rank %d is not a multiple of 8 up to %d", r, kMaxRank);
-  if (C < 8 || C % 8 || ld_z % 8) return ixh::fail(ixh::IX_EARG, "lora: width %d and its row stride must be multiples of 8", C);
-  GradArgs a;
-  a.h = static_cast<const __nv_bfloat16*>(h);
-  a.z = static_cast<const __nv_bfloat16*>(z);
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.perm = static_cast<const int*>(perm);
-  a.offsets = static_cast<const int*>(offsets);
-  a.ld_z = ld_z;
-  a.T = T, a.C = C, a.r = r, a.by_cols = by_cols;
-  const int tiles = (C + kCols - 1) / kCols;
+namespace {
+
+// One factor's gradient.
+int factor_grad(const GradArgs& a, int E, cudaStream_t s) {
+  const int T = a.T, r = a.r, tiles = (a.C + kCols - 1) / kCols;
   if (T <= 0) {
-    IX_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(E) * r * C * 2, reinterpret_cast<cudaStream_t>(stream)));
+    IX_CUDA(cudaMemsetAsync(a.out, 0, static_cast<size_t>(E) * r * a.C * 2, s));
     return 0;
   }
   // CTAs an adapter's columns: until the card has two a multiprocessor, but not beyond four tiles of an average adapter's
   // tokens each (8192 tokens x 24576: 79 us with 2, 117 with 1, 84 with 4; 463 tokens an adapter: 8 us with 2, 11 with 4)
   int c = 1;
-  while (c < 8 && tiles * E * c < 148 * 2 && T / E > c * 4 * kTok) c *= 2;
+  while (c < 8 && static_cast<long long>(tiles) * E * c < 148 * 2 && T / E > c * 4 * kTok) c *= 2;
   const dim3 grid(c, tiles, E);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (r <= 8) return launch_cluster(lora_grad_kernel<1>, a, grid, c, grad_smem<1>(), s);
   if (r <= 16) return launch_cluster(lora_grad_kernel<2>, a, grid, c, grad_smem<2>(), s);
   if (r <= 32) return launch_cluster(lora_grad_kernel<4>, a, grid, c, grad_smem<4>(), s);
   if (r <= 64) return launch_cluster(lora_grad_kernel<8>, a, grid, c, grad_smem<8>(), s);
   return launch_cluster(lora_grad_kernel<16>, a, grid, c, grad_smem<16>(), s);
+}
+
+}  // namespace
+
+// Backward of out = y + s (x A^T) B^T: g = s dy B, dx = base + g A (dx null: not wanted; base null: zero), dA = g^T x and
+// dB = dy^T h by adapter (null: not wanted; zero for an adapter without tokens). h: what ix_lora_apply stored; g: bf16 [2, T, r]
+// scratch, needed for dA. dx may be base.
+IX_API int ix_lora_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* base, long long ld_base, void* dx,
+                            long long ld_dx, const void* A, const void* B, const void* scale, const void* perm, const void* tiles_small,
+                            const void* tiles_large, const void* n_tiles, const void* offsets, const void* h, void* g, void* dA, void* dB, int T,
+                            int K, int N, int r, int E, void* stream) {
+  if (T > 0 && dA != nullptr && g == nullptr) return ixh::fail(ixh::IX_EARG, "lora: the gradient of A needs scratch for g");
+  if (T > 0 && dB != nullptr && h == nullptr) return ixh::fail(ixh::IX_EARG, "lora: the gradient of B needs the forward's h");
+  if (r < 8 || r > kMaxRank || r % 8) return ixh::fail(ixh::IX_EARG, "lora: rank %d is not a multiple of 8 up to %d", r, kMaxRank);
+  if (K < 8 || N < 8 || K % 8 || N % 8 || ld_dy % 8 || ld_x % 8) return ixh::fail(ixh::IX_EARG, "lora: widths and row strides must be multiples of 8");
+  if (dx != nullptr || dA != nullptr) {
+    const int rc = ix_lora_apply(dy, ld_dy, base, ld_base, dx, ld_dx, B, A, scale, perm, tiles_small, tiles_large, n_tiles, dA != nullptr ? g : nullptr,
+                                 T, N, K, r, E, 1, stream);
+    if (rc) return rc;
+  }
+  // (both in one launch were 126 us at 8192 tokens x 4096 and 24576 instead of 107: the one cut into parts suits only one)
+  GradArgs a = {};
+  a.perm = static_cast<const int*>(perm), a.offsets = static_cast<const int*>(offsets);
+  a.T = T, a.r = r;
+  int rc = 0;
+  if (dB != nullptr) {
+    a.h = static_cast<const __nv_bfloat16*>(h), a.z = static_cast<const __nv_bfloat16*>(dy), a.out = static_cast<__nv_bfloat16*>(dB);
+    a.ld_z = ld_dy, a.C = N, a.by_cols = 1;
+    rc = factor_grad(a, E, reinterpret_cast<cudaStream_t>(stream));
+  }
+  if (rc == 0 && dA != nullptr) {
+    a.h = static_cast<const __nv_bfloat16*>(g), a.z = static_cast<const __nv_bfloat16*>(x), a.out = static_cast<__nv_bfloat16*>(dA);
+    a.ld_z = ld_x, a.C = K, a.by_cols = 0;
+    rc = factor_grad(a, E, reinterpret_cast<cudaStream_t>(stream));
+  }
+  return rc;
 }

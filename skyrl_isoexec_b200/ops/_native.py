@@ -56,7 +56,7 @@ _SIGS = {
     "ix_lora_max_tiles": [_I, _I, _I],
     "ix_lora_plan": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
     "ix_lora_apply": [_P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
-    "ix_lora_grad": [_P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P],
+    "ix_lora_backward": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P],
     "ix_tensor_adamw_chunk": [],
     "ix_tensor_adamw": [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _D, _D, _D, _D, _L, _P],
     "ix_accum_bf16_to_f32": [_P, _P, _L, _I, _P],

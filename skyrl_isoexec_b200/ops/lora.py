@@ -124,16 +124,6 @@ def _apply(x, base, out, down, up, scale, plan, across, want_h):
     return h
 
 
-def _factor_grad(h, z, like, plan, by_cols):
-    out = torch.empty_like(like, memory_format=torch.contiguous_format)
-    r, C = (like.shape[2], like.shape[1]) if by_cols else (like.shape[1], like.shape[2])
-    _native.check(
-        _native.lib().ix_lora_grad(h.data_ptr(), z.data_ptr(), z.stride(0), out.data_ptr(), plan._apply_args[0], plan._offsets_ptr,
-                                   plan.T, C, r, plan.E, int(by_cols), _native.raw_stream(z.get_device())),
-        "ix_lora_grad")
-    return out
-
-
 def _cpu_h(x, A, scale, plan):
     """s (x A^T) of every token with its own adapter, fp32 [T, r]; zero rows without one."""
     h = torch.zeros(x.shape[0], A.shape[1])
@@ -172,14 +162,20 @@ def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, nee
     dx = dA = dB = None
     if x.is_cuda:
         with _device_of(x):
-            g = None
-            if need_x or need_a:
-                dx = None if not need_x else base if base is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                g = _apply(dy, base if need_x else None, dx, B, A, scale, plan, True, need_a)
-            if need_a:
-                dA = _factor_grad(g, x, A, plan, False)
-            if need_b:
-                dB = _factor_grad(h, dy, B, plan, True)
+            (T, K), (E, N, r) = x.shape, B.shape
+            if need_x:
+                dx = base if base is not None else torch.empty(T, K, dtype=x.dtype, device=x.device)
+            dA = torch.empty(E, r, K, dtype=x.dtype, device=x.device) if need_a else None
+            dB = torch.empty(E, N, r, dtype=x.dtype, device=x.device) if need_b else None
+            g = torch.empty(2, T, r, dtype=x.dtype, device=x.device) if need_a else None
+            base = base if need_x else None
+            _native.check(
+                _native.lib().ix_lora_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _native.ptr(base),
+                                               base.stride(0) if base is not None else 0, _native.ptr(dx), dx.stride(0) if dx is not None else 0,
+                                               A.data_ptr(), B.data_ptr(), scale.data_ptr(), *plan._apply_args, plan._offsets_ptr,
+                                               _native.ptr(h) if need_b else None, _native.ptr(g), _native.ptr(dA), _native.ptr(dB), T, K, N, r, E,
+                                               _native.raw_stream(x.get_device())),
+                "ix_lora_backward")
         return dx, dA, dB
     g = _cpu_h(dy, B.transpose(1, 2), scale, plan)
     if need_x:
@@ -192,6 +188,12 @@ def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, nee
     return dx, dA, dB
 
 
+def _first_order_only() -> None:
+    # (what autograd's decorator for this does, without the 15 us that it costs a call)
+    if torch.is_grad_enabled():
+        raise RuntimeError("lora: the backward pass is not differentiable itself (create_graph=True)")
+
+
 class _LoraAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, A, B, scale, plan):
@@ -202,8 +204,8 @@ class _LoraAdd(torch.autograd.Function):
         return out.view(y.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _first_order_only()
         x, A, B, scale, h = ctx.saved_tensors
         ny, nx, na, nb = ctx.needs_input_grad[:4]
         dx, dA, dB = _backward(_rows(dout), x, A, B, scale, h, ctx.plan, None, nx, na, nb)
@@ -220,8 +222,8 @@ class _LoraLinear(torch.autograd.Function):
         return out.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _first_order_only()
         x, w, A, B, scale, h = ctx.saved_tensors
         nx, nw, na, nb = ctx.needs_input_grad[:4]
         dy = _rows(dout)

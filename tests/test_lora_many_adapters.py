@@ -242,10 +242,14 @@ def test_refusals_on_a_gpu():
     for call, words in bad:
         with pytest.raises(ValueError, match=words):
             call()
-    out = lora_add(y, x, A.requires_grad_(True), B, scale, plan)
-    (dA,) = torch.autograd.grad(out.sum(), A, create_graph=True)
-    with pytest.raises(RuntimeError):
-        dA.sum().backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_derivatives_are_refused(dev):
+    y, x, A, B, scale, ids, _ = _make(10, 16, 24, 8, 2, "shuffled", dev)
+    out = lora_add(y, x, A.requires_grad_(True), B, scale, LoraPlan(ids, 2))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(out.sum(), A, create_graph=True)
 
 
 @pytest.mark.gpu
