@@ -948,12 +948,13 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   a.n_tiles = static_cast<const int*>(n_tiles) + large;
   const int tiles = bound_tiles(T, E, large ? kLarge : kSmall);
   if (tiles > 65535) return ixh::fail(ixh::IX_ESIZE, "lora: %d tokens of %d adapters make more than 65535 tiles", T, E);
-  // CTAs a tile: until the card has three a multiprocessor, but not beyond eight steps (small: one a warp) each; where a CTA
-  // then still has 96 stages, once more: the last CTAs to run are shorter (8192 x 4096 -> 24576: 189 us with 4, 163 with 8;
-  // 4096 -> 4096, with 32 stages: 44 us either way, but rank 64 loses from 66 to 77)
+  // CTAs a tile: as many as run together, but not beyond eight steps (small: one a warp) each; where a large tile's CTA then
+  // still has 96 stages, once more: the last CTAs to run are shorter (8192 x 4096 -> 24576: 189 us with 4, 163 with 8; with 32
+  // stages each, 44 us either way, and rank 64 loses from 66 to 77)
   int c = 1;
   const int widest = (K > N ? K : N) / 32;
-  while (c < 8 && tiles * c < 148 * 3 && widest > c * 8) c *= 2;
+  const int together = 148 * (!large || r <= 16 ? 4 : r <= 32 ? 3 : r <= 64 ? 2 : 1);
+  while (c < 8 && tiles * c * 2 <= together && widest > c * 8) c *= 2;
   if (large && c < 8 && (K + N) / 64 >= 96 * c) c *= 2;
   const dim3 grid(c, tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -9,8 +9,6 @@ different ranks share a bank when the smaller ones are filled up with zero rows 
 
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 
 from . import _native
@@ -29,7 +27,7 @@ class LoraPlan:
             raise ValueError(f"LoraPlan: ids are a flat int32 or int64 tensor, not {tuple(ids.shape)} {ids.dtype}")
         if num_adapters < 1:
             raise ValueError("LoraPlan: at least one adapter")
-        self.T, self.E, self.device = ids.shape[0], int(num_adapters), ids.device
+        self.T, self.E, self.device, self.index = ids.shape[0], int(num_adapters), ids.device, ids.get_device()
         if not ids.is_cuda:
             self.ids = ids.clone()
             return
@@ -97,29 +95,28 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _factor(t: torch.Tensor) -> torch.Tensor:
     if not t.is_contiguous():
         t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def _device_of(x: torch.Tensor):
-    """Makes x's device current; nothing where it is (the usual case, and microseconds of a small call)."""
-    return nullcontext() if torch.cuda.current_device() == x.get_device() else torch.cuda.device(x.device)
-
-
-def _apply(x, base, out, down, up, scale, plan, across, want_h):
-    """csrc/lora.cu::ix_lora_apply on prepared operands; returns h [2, T, r] in the plan's order if wanted."""
+def _apply(x, base, out, down, up, scale, plan, want_h):
+    """out = base + s (x down^T) up^T on prepared operands (csrc/lora.cu::ix_lora_apply); returns h [2, T, r] in the plan's order
+    if wanted."""
     T, K = x.shape
-    E = plan.E
-    r, N = (down.shape[1], up.shape[1]) if not across else (down.shape[2], up.shape[2])
+    (E, r, _), N = down.shape, up.shape[1]
     h = torch.empty(2, T, r, dtype=torch.bfloat16, device=x.device) if want_h else None
     if T == 0:
         return h
     _native.check(
-        _native.lib().ix_lora_apply(x.data_ptr(), x.stride(0), _native.ptr(base), base.stride(0) if base is not None else 0, _native.ptr(out),
-                                    out.stride(0) if out is not None else 0, down.data_ptr(), up.data_ptr(), scale.data_ptr(),
-                                    *plan._apply_args, _native.ptr(h), T, K, N, r, E, int(across), _native.raw_stream(x.get_device())),
+        _native.lib().ix_lora_apply(x.data_ptr(), x.stride(0), base.data_ptr(), base.stride(0), out.data_ptr(), out.stride(0), down.data_ptr(),
+                                    up.data_ptr(), scale.data_ptr(), *plan._apply_args, None if h is None else h.data_ptr(), T, K, N, r, E, 0,
+                                    _native.raw_stream(plan.index)),
         "ix_lora_apply")
     return h
 
@@ -148,9 +145,11 @@ def _cpu_grad(h, z, plan):
 def _forward(y, x, A, B, scale, plan, inplace: bool, want_h: bool):
     """(out, h) on rows; ``inplace``: out is y."""
     if x.is_cuda:
-        with _device_of(x):
-            out = y if inplace else torch.empty(y.shape, dtype=y.dtype, device=y.device)
-            return out, _apply(x, y, out, A, B, scale, plan, False, want_h)
+        out = y if inplace else torch.empty_like(y, memory_format=torch.contiguous_format)
+        if torch.cuda.current_device() == plan.index:        # (the usual case: no context manager in a small call)
+            return out, _apply(x, y, out, A, B, scale, plan, want_h)
+        with torch.cuda.device(plan.index):
+            return out, _apply(x, y, out, A, B, scale, plan, want_h)
     h = _cpu_h(x, A, scale, plan)
     hit = ((plan.ids >= 0) & (plan.ids < plan.E))[:, None]
     out = torch.where(hit, (y.float() + _cpu_up(h, B, plan)).to(y.dtype), y)
@@ -161,7 +160,7 @@ def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, nee
     """(dx, dA, dB); ``base``: the other part of dx, added to in place."""
     dx = dA = dB = None
     if x.is_cuda:
-        with _device_of(x):
+        with torch.cuda.device(plan.index):
             (T, K), (E, N, r) = x.shape, B.shape
             if need_x:
                 dx = base if base is not None else torch.empty(T, K, dtype=x.dtype, device=x.device)
@@ -237,6 +236,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     """``y + s_a (x A_a^T) B_a^T`` for every token's own adapter: x [..., K], y [..., N], A [E, r, K], B [E, N, r], scale [E].
     One rounding, of the result; a token without an adapter gets y's bits. Differentiable in y, x, A and B."""
     _check(y, x, A, B, scale, plan)
+    scale = _flat(scale)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or y.requires_grad):
         return _LoraAdd.apply(y, x, A, B, scale, plan)
     out = _forward(_rows(y), _rows(x), _factor(A), _factor(B), scale, plan, False, False)[0]
@@ -249,6 +249,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, A: torch.Tensor, B: torch.Tens
     _check(None, x, A, B, scale, plan)
     if w.dim() != 2 or w.shape != (B.shape[1], A.shape[2]) or w.dtype != x.dtype or w.device != x.device:
         raise ValueError(f"lora: w {tuple(w.shape)} {w.dtype} does not fit factors of widths {A.shape[2]} and {B.shape[1]}")
+    scale = _flat(scale)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or w.requires_grad):
         return _LoraLinear.apply(x, w, A, B, scale, plan)
     x2 = _rows(x)

@@ -149,6 +149,9 @@ def test_strides_leading_dimensions_and_neighbours(dev):
         kept = wide_y.clone()
         assert torch.equal(lora_add(wide_y[:, off:off + N], wide_x[:, off:off + K], A, B, scale, plan), want)
         assert torch.equal(wide_y.nan_to_num(7.0), kept.nan_to_num(7.0))
+    spaced = torch.full((2 * E,), float("nan"), device=dev)
+    spaced[::2] = scale
+    assert torch.equal(lora_add(y, x, A, B, spaced[::2], plan), want)
     assert torch.equal(lora_add(y.view(3, 20, N), x.view(3, 20, K), A, B, scale, plan), want.view(3, 20, N))
     one = x[:1].expand(T, K)
     assert torch.equal(lora_add(y, one, A, B, scale, plan), lora_add(y, one.contiguous(), A, B, scale, plan))
