@@ -526,13 +526,20 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT <= 4 ? 3 : RT <= 8 ? 2 :
     uint32_t a[2][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) ldsm4(st + wide_at(mt * 16 + l8 + 8 * (lm & 1), hf * 4 + 2 * s + (lm >> 1)), a[s]);
+    // products that add to the same sums stand apart: one waits 23 cycles for the other
+    constexpr int kGroup = RT < 8 ? RT : 8;
 #pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      uint32_t b[4];
-      if constexpr (ACROSS) ldsm4t(fs + narrow_at<RT>(hf * 32 + lm * 8 + l8, j), b);
-      else ldsm4(fs + wide_at(j * 8 + l8, hf * 4 + lm), b);
-      mma16816(acc[j], a[0][0], a[0][1], a[0][2], a[0][3], b[0], b[1]);
-      mma16816(acc[j], a[1][0], a[1][1], a[1][2], a[1][3], b[2], b[3]);
+    for (int j0 = 0; j0 < RT; j0 += kGroup) {
+      uint32_t b[kGroup][4];
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+        if constexpr (ACROSS) ldsm4t(fs + narrow_at<RT>(hf * 32 + lm * 8 + l8, j0 + j), b[j]);
+        else ldsm4(fs + wide_at((j0 + j) * 8 + l8, hf * 4 + lm), b[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) mma16816(acc[j0 + j], a[0][0], a[0][1], a[0][2], a[0][3], b[j][0], b[j][1]);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) mma16816(acc[j0 + j], a[1][0], a[1][1], a[1][2], a[1][3], b[j][2], b[j][3]);
     }
     st = st == ring + (kRing - 1) * tile_stage<RT>() ? ring : st + tile_stage<RT>();
   }
@@ -641,21 +648,22 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT <= 4 ? 3 : RT <= 8 ? 2 :
         uint32_t b[4];
         fetch(factor(lm & 1, j + (lm >> 1)), b);
         mma16816(o[j], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b[0], b[1]);
-        mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[0], b[1]);
         mma16816(o[j + 1], hi[0][0], hi[0][1], hi[0][2], hi[0][3], b[2], b[3]);
+        mma16816(o[j], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[0], b[1]);
         mma16816(o[j + 1], lo[0][0], lo[0][1], lo[0][2], lo[0][3], b[2], b[3]);
       }
     } else {
 #pragma unroll
       for (int q = 0; q < RT / 4; ++q) {
+        uint32_t b[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b[4];
-          fetch(factor(4 * q + lm, j), b);
-          mma16816(o[j], hi[2 * q][0], hi[2 * q][1], hi[2 * q][2], hi[2 * q][3], b[0], b[1]);
-          mma16816(o[j], lo[2 * q][0], lo[2 * q][1], lo[2 * q][2], lo[2 * q][3], b[0], b[1]);
-          mma16816(o[j], hi[2 * q + 1][0], hi[2 * q + 1][1], hi[2 * q + 1][2], hi[2 * q + 1][3], b[2], b[3]);
-          mma16816(o[j], lo[2 * q + 1][0], lo[2 * q + 1][1], lo[2 * q + 1][2], lo[2 * q + 1][3], b[2], b[3]);
+        for (int j = 0; j < 4; ++j) fetch(factor(4 * q + lm, j), b[j]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16816(o[j], hi[2 * q + k][0], hi[2 * q + k][1], hi[2 * q + k][2], hi[2 * q + k][3], b[j][2 * k], b[j][2 * k + 1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16816(o[j], lo[2 * q + k][0], lo[2 * q + k][1], lo[2 * q + k][2], lo[2 * q + k][3], b[j][2 * k], b[j][2 * k + 1]);
         }
       }
     }
@@ -806,15 +814,18 @@ __global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ 
       uint32_t za[2][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m) ldsm4t(st + (k + l8 + 8 * (lm >> 1)) * kZRow + (cg4 * 32 + m * 16 + 8 * (lm & 1)) * 2, za[m]);
+      constexpr int kGroup = RT < 4 ? RT : 4;
 #pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        uint32_t b[4];                                 // (hi, lo) x (tokens k..k+7 | k+8..k+15)
-        ldsm4t(hs + (lm >> 1) * kTok * 16 * RT + narrow_at<RT>(k + l8 + 8 * (lm & 1), j), b);
+      for (int j0 = 0; j0 < RT; j0 += kGroup) {
+        uint32_t b[kGroup][4];                         // (hi, lo) x (tokens k..k+7 | k+8..k+15)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma16816(acc[m][j], za[m][0], za[m][1], za[m][2], za[m][3], b[0], b[1]);
-          mma16816(acc[m][j], za[m][0], za[m][1], za[m][2], za[m][3], b[2], b[3]);
-        }
+        for (int j = 0; j < kGroup; ++j) ldsm4t(hs + (lm >> 1) * kTok * 16 * RT + narrow_at<RT>(k + l8 + 8 * (lm & 1), j0 + j), b[j]);
+#pragma unroll
+        for (int u = 0; u < 4; u += 2)
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) mma16816(acc[m][j0 + j], za[m][0], za[m][1], za[m][2], za[m][3], b[j][u], b[j][u + 1]);
       }
     }
   }
