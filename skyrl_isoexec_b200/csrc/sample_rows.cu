@@ -45,6 +45,7 @@ struct Args {
   float* logprobs;
   int* marked;                        // rows the first kernel leaves to the second (null: all rows are the second's)
   int cached;                         // a CTA's pieces stay in shared memory after the first pass
+  int kept;                           // room for them, in pieces
 };
 
 template <typename T>
@@ -734,6 +735,7 @@ struct Step {                         // what rank 0 tells the cluster
   unsigned prefix;
 };
 constexpr int kList = 1024;
+constexpr int kAlive = 512;           // a warp's places for tokens in the window
 // Whether a search ends in the n tokens that stand behind cc others (weights in units: mm before them, next behind them).
 // 0: the end-th token. 1: the last that begin in front of the aim and among the first `end`. 2: the last that begin at or
 // in front of it. Exactly one of a row's bins, or of a bin's values, says yes: the sums are whole numbers.
@@ -760,6 +762,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   __shared__ unsigned dcnt[256], dlow[256], dhigh[256];
   __shared__ Shared sh;
   __shared__ Step step[3][5];
+  float* const alive = reinterpret_cast<float*>(kept_pieces + a.kept);        // behind the row's pieces
   __shared__ unsigned list[kList], list_n;
   __shared__ u64 list_units[kList];
   __shared__ double table[64];
@@ -796,8 +799,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   const auto units = [&](float x) { return x == top ? static_cast<u64>(kUnit) : units_of((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
   const double floor_units = row.min_p * kUnit;
   unsigned some = 0;
-  s.each([&](float x) {
-    if (!(x >= low)) return;
+  const auto count_in = [&](float x) {
     const u64 q = units(x);
     const int b = bin_of(x);
     atomicAdd(&cnt[b], 1u);
@@ -805,7 +807,65 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     // on the border itself (a unit is 2^-44) the weight decides
     if (row.min_p > 0.0) some += fabs(static_cast<double>(q) - floor_units) > 2.0 ? static_cast<double>(q) > floor_units : weight(x, top, row.T) >= row.min_p;
     else ++some;
+  };
+  // A warp gathers what lies in the window and counts it in full groups of 32: a masked row's work in 64 bits is that of the
+  // tokens its mask leaves. Where all of them fit, the searches look at these instead of at the row again.
+  float* const mine = alive + (tid >> 5) * kAlive;
+  const int lane = tid & 31;
+  int have = 0, done = 0, seen_tokens = 0;
+  bool all_kept = true, dense = false;
+  s.edges([&](T x) {
+    if (value_of<T>(x) >= low) count_in(value_of<T>(x));
   });
+  for (int i0 = s.lo + (tid & ~31); i0 < s.hi; i0 += 2 * kThreads) {
+    uint4 w[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (i0 + u * kThreads + lane < s.hi) w[u] = s.piece(i0 + u * kThreads + lane);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool in = i0 + u * kThreads + lane < s.hi;
+      const T* x = reinterpret_cast<const T*>(&w[u]);
+      if (dense) {                                      // most tokens are in the window: gathering them costs more than it saves
+#pragma unroll
+        for (int q = 0; q < Share<T>::kPer; ++q)
+          if (in && value_of<T>(x[q]) >= low) count_in(value_of<T>(x[q]));
+        continue;
+      }
+      seen_tokens += 32 * Share<T>::kPer;
+#pragma unroll
+      for (int q = 0; q < Share<T>::kPer; ++q) {
+        const float v = in ? value_of<T>(x[q]) : 0.f;
+        const bool ok = in && v >= low;
+        const unsigned m = __ballot_sync(0xffffffffu, ok);
+        if (ok) mine[have + __popc(m & ((1u << lane) - 1u))] = v;
+        have += __popc(m);
+      }
+      __syncwarp();
+      for (; have - done >= 32; done += 32) count_in(mine[done + lane]);
+      if (have > kAlive - 32 * Share<T>::kPer) {        // no room for another piece: only what is not counted yet stays
+        const float v = done + lane < have ? mine[done + lane] : 0.f;
+        __syncwarp();
+        if (done + lane < have) mine[lane] = v;
+        __syncwarp();
+        if (all_kept) dense = 2 * have > seen_tokens;
+        have -= done, done = 0, all_kept = false;
+      }
+    }
+  }
+  if (done + lane < have) count_in(mine[done + lane]);
+  const auto each_alive = [&](auto&& f) {
+    if (!all_kept) {
+      s.each([&](float x) {
+        if (x >= low) f(x);
+      });
+      return;
+    }
+    s.edges([&](T x) {
+      if (value_of<T>(x) >= low) f(value_of<T>(x));
+    });
+    for (int j = lane; j < have; j += 32) f(mine[j]);
+  };
   some = warp_all(some, Add());
   if ((tid & 31) == 0) sh.sc[tid >> 5] = some;
   __syncthreads();
@@ -889,8 +949,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       // the bin's tokens in a list of rank 0; each finds what stands in front of it by looking at all the others
       unsigned* to = cl.map_shared_rank(list, 0);
       unsigned* at = cl.map_shared_rank(&list_n, 0);
-      s.each([&](float x) {
-        if (x >= low && bin_of(x) == first.bin) to[atomicAdd(at, 1u)] = order_key(x);
+      each_alive([&](float x) {
+        if (bin_of(x) == first.bin) to[atomicAdd(at, 1u)] = order_key(x);
       });
       cl.sync();
       if (rank == 0) {
@@ -919,8 +979,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       const int shift = 24 - 8 * level;
       if (tid < 256) dcnt[tid] = 0u, dlow[tid] = 0u, dhigh[tid] = 0u;
       __syncthreads();
-      s.each([&](float x) {
-        if (!(x >= low) || bin_of(x) != first.bin) return;
+      each_alive([&](float x) {
+        if (bin_of(x) != first.bin) return;
         const unsigned k = order_key(x);
         if (level > 0 && (k >> (shift + 8)) != prefix) return;
         atomicAdd(&dcnt[(k >> shift) & 255u], 1u);
@@ -1031,12 +1091,20 @@ IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int
   // tokens each. Where its pieces then fit beside another CTA's, they stay in shared memory after the first pass
   int c = 1;
   while (c < kMaxCluster && rows * c * 2 <= 148 * 2 && V > c * 8192) c *= 2;
-  const long long bytes = (static_cast<long long>(V) * (dtype == 0 ? 2 : 4) / c + 32 + 15) / 16 * 16;
-  a.cached = bytes <= (static_cast<long long>(rows) * c <= 148 ? 160 : 60) * 1024;
-  const int smem = a.cached ? static_cast<int>(bytes) : 0;
+  const int pieces = static_cast<int>(static_cast<long long>(V) * (dtype == 0 ? 2 : 4) / c / 16 + 2);
+  const bool alone = static_cast<long long>(rows) * c <= 148;          // one CTA a multiprocessor
+  const auto fits = [&](int other) { return pieces * 16 <= (alone ? 220 : 106) * 1024 - other; };
+  constexpr int kAnyStatic = 44 * 1024, kFew = kWarps * kAlive * 4, kBf16Static = 20 * 1024;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == 1) return launch(sample_any_kernel<float>, a, rows, c, smem, false, s);
-  const int rc = launch(sample_bf16_kernel, a, rows, c, smem, false, s);
+  const auto any = [&](void (*kern)(Args), bool early) {
+    a.cached = fits(kAnyStatic + kFew);
+    a.kept = a.cached ? pieces : 0;
+    return launch(kern, a, rows, c, a.kept * 16 + kFew, early, s);
+  };
+  if (dtype == 1) return any(sample_any_kernel<float>, false);
+  a.cached = fits(kBf16Static);
+  a.kept = a.cached ? pieces : 0;
+  const int rc = launch(sample_bf16_kernel, a, rows, c, a.kept * 16, false, s);
   // started while the first one drains: it waits for its marks, and nearly always ends there
-  return rc ? rc : launch(sample_any_kernel<__nv_bfloat16>, a, rows, c, smem, true, s);
+  return rc ? rc : any(sample_any_kernel<__nv_bfloat16>, true);
 }
