@@ -192,7 +192,8 @@ struct Row {                          // what a row asks for
     const float p = a.top_p ? a.top_p[r] : 1.f, m = a.min_p ? a.min_p[r] : 0.f;
     top_p = p < 1.f ? static_cast<double>(p) : 2.0;     // 2: off (so is what is not a number)
     min_p = m > 0.f ? static_cast<double>(m) : 0.0;
-    u = a.u[r];
+    const float v = a.u[r];
+    u = v > 0.f ? fminf(v, 0.99999994f) : 0.f;          // the numbers are of [0, 1): what is not, or is no number, is moved there
   }
 };
 
@@ -1068,7 +1069,7 @@ int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem
 
 IX_API int ix_sample_rows_max_vocab() { return 1 << 19; }
 
-// logits [rows, V] with row stride ld, dtype 0 = bf16, 1 = fp32; u fp32 [rows] in [0, 1); temperature / top_p / min_p fp32
+// logits [rows, V] with row stride ld, dtype 0 = bf16, 1 = fp32; u fp32 [rows] in [0, 1), others are clamped; temperature / top_p / min_p fp32
 // [rows], top_k int32 [rows] (each may be null); tokens int64 [rows], logprobs fp32 [rows]; marked int32 [rows] scratch (bf16).
 IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int dtype, const void* u, const void* temperature, const void* top_k,
                           const void* top_p, const void* min_p, void* tokens, void* logprobs, void* marked, void* stream) {

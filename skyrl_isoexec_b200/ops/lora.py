@@ -90,7 +90,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     st = t.stride()
     if (st[1] != 1 or st[0] % 8 or t.data_ptr() % 16) and t.shape[0]:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.stride(0) % 8 or t.data_ptr() % 16:            # (a single row is contiguous whatever its stride says)
             t = t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -31,7 +31,8 @@ class TensorAdamW:
 
     Gradients are read from ``grads``, one buffer per parameter that the program fills again for every step (autograd, a
     projection, ``F.gemm_tn(out=...)``); without the argument they are made here, fp32 zeros in one allocation
-    (``zero_grad`` clears them). The buffers are fixed at construction: a step does no per-tensor work on the host.
+    (``zero_grad`` clears them). The memory of parameters and gradients is fixed at construction (and kept alive): a step does
+    no per-tensor work on the host, and does not see a ``p.data`` that was replaced.
 
     ``state_bits=8``: both moments in e4m3 with one scale per 256 elements, the second by its square root, 2 bytes and a bit
     per element instead of 8. ``state`` holds flat buffers in which tensor ``i`` starts at ``offsets[i]`` (a multiple of
@@ -77,6 +78,7 @@ class TensorAdamW:
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("TensorAdamW: two of the parameters share memory")
+        self._memory = [t.detach() for t in (*params, *self.grads)]      # what a step writes and reads stays allocated
         self.step_count = 0
         st = FP8 if state_bits == 8 else torch.float32
         self.state = {"exp_avg": torch.zeros(total, dtype=st, device=dev), "exp_avg_sq": torch.zeros(total, dtype=st, device=dev)}

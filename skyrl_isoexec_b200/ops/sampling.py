@@ -26,7 +26,7 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor
                 top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(tokens int64 [rows], log-probabilities fp32 [rows]).
 
-    ``logits`` [rows, V] bf16 or fp32 with unit inner stride; ``u`` fp32 [rows] in ``[0, 1)``. ``temperature`` fp32 (default
+    ``logits`` [rows, V] bf16 or fp32; ``u`` fp32 [rows] in ``[0, 1)`` (a number outside is moved to the nearer end, NaN to 0). ``temperature`` fp32 (default
     1; at or below 0: the largest logit), ``top_k`` int32 (at or below 0: off), ``top_p`` fp32 (1 or more: off), ``min_p`` fp32 (at
     or below 0: off), each [rows] or None. A logit of -inf or NaN is never drawn; a row that has no other gives token 0 with
     log-probability -inf. The log-probability is that of the token in the kept, renormalised distribution, the one it was
@@ -79,6 +79,7 @@ def _sample_cpu(logits, u, temperature, top_k, top_p, min_p):
     one, off = torch.ones(rows), torch.zeros(rows)
     x = logits.float()
     x = torch.where(x.isnan(), float("-inf"), x) + 0.0
+    u = u.nan_to_num(0.0).clamp(0.0, 1.0 - 2.0 ** -24)
     vals, order = torch.sort(x, dim=-1, descending=True, stable=True)
     vals = vals.double()
     top = vals[:, :1]

@@ -153,6 +153,10 @@ def test_strides_leading_dimensions_and_neighbours(dev):
     spaced[::2] = scale
     assert torch.equal(lora_add(y, x, A, B, spaced[::2], plan), want)
     assert torch.equal(lora_add(y.view(3, 20, N), x.view(3, 20, K), A, B, scale, plan), want.view(3, 20, N))
+    odd = torch.full((2, K + 9), float("nan"), device=dev).bfloat16()      # a single row: contiguous, with a stride of K + 9
+    odd[0, 8:8 + K] = x[3]
+    p1 = LoraPlan(ids[3:4], E)
+    assert torch.equal(lora_add(y[3:4], odd[:1, 8:8 + K], A, B, scale, p1), want[3:4])
     one = x[:1].expand(T, K)
     assert torch.equal(lora_add(y, one, A, B, scale, plan), lora_add(y, one.contiguous(), A, B, scale, plan))
     At, Bt = A.transpose(1, 2).contiguous().transpose(1, 2), B.transpose(1, 2).contiguous().transpose(1, 2)

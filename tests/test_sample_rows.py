@@ -146,6 +146,10 @@ def test_masks_infinities_and_nan(dev, dtype):
         assert tokens[0] == 0 and lps[0] == -inf and tokens[1] == 0 and tokens[2] == 1234
         assert (tokens >= 0).all() and (tokens < V).all()
     _check(x, u, T=0.0)
+    # numbers outside [0, 1) are moved to its ends
+    for bad, good in ((-0.5, 0.0), (1.0, 1 - 2.0 ** -24), (7.0, 1 - 2.0 ** -24), (nan, 0.0), (inf, 1 - 2.0 ** -24), (-inf, 0.0)):
+        b, g = (torch.full((12,), v, device=dev) for v in (bad, good))
+        assert all(torch.equal(s, t) for s, t in zip(sample_rows(x, b), sample_rows(x, g)))
     # settings that are no numbers are off, a temperature that is none is greedy
     for name in ("p", "m"):
         assert torch.equal(_check(x, u, **{name: nan})[0], _check(x, u)[0])

@@ -148,6 +148,18 @@ def test_refusals():
     assert opt.step_count == 0
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_replaced_storage_is_neither_stepped_nor_freed(dev):
+    w = torch.ones(300, device=dev)
+    opt = TensorAdamW([w], grads=[torch.ones(300, device=dev)], lr=0.1)
+    w.data = torch.zeros(300, device=dev)
+    junk = [torch.zeros(300, device=dev) for _ in range(8)]
+    if dev == "cuda":
+        opt.step()
+        torch.cuda.synchronize()
+        assert not w.any() and not any(j.any() for j in junk)
+
+
 @pytest.mark.gpu
 def test_another_stream_capture_refused_and_version_counters():
     torch.manual_seed(2)
