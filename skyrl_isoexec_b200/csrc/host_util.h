@@ -9,6 +9,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
 #include <mutex>
 #include <unordered_map>
 
@@ -57,6 +58,43 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+// Launch in clusters of `cluster` CTAs along x, with up to `most` bytes of dynamic shared memory. The kernel's limit is raised
+// to `most` once per device (a microsecond of every call otherwise). `early`: programmatic stream serialization, as above.
+template <auto Kern, typename Args>
+inline int launch_cluster(const Args& args, dim3 grid, int threads, int cluster, int smem, int most, bool early, cudaStream_t stream) {
+  if (most > 0) {
+    static std::atomic<unsigned long long> raised{0ull};
+    int dev = 0;
+    IX_CUDA(cudaGetDevice(&dev));
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev >= 64 || !(raised.load(std::memory_order_acquire) & bit)) {
+      IX_CUDA(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+      raised.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {                   // (a CTA by itself is a cluster of one without the attribute)
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster, at[n].val.clusterDim.y = 1, at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (early && pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  IX_CUDA(cudaLaunchKernelEx(&cfg, Kern, args));
+  return 0;
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -882,29 +882,17 @@ __global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-template <typename Args>
-int launch_cluster(void (*kern)(Args), const Args& args, dim3 grid, int cluster, int smem, cudaStream_t s) {
-  if (smem > 48 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  IX_CUDA(cudaLaunchKernelEx(&cfg, kern, args));
-  return 0;
+template <auto Kern, typename Args>
+int launch(const Args& args, dim3 grid, int smem, cudaStream_t s) {
+  return ixh::launch_cluster<Kern>(args, grid, 256, grid.x, smem, smem, false, s);
 }
 
 template <int RT>
 int apply_tile(const ApplyArgs& a, int large, int across, dim3 grid, cudaStream_t s) {
-  if (large && across) return launch_cluster(lora_tile_kernel<RT, true>, a, grid, grid.x, tile_smem<RT>(), s);
-  if (large) return launch_cluster(lora_tile_kernel<RT, false>, a, grid, grid.x, tile_smem<RT>(), s);
-  if (across) return launch_cluster(lora_apply_kernel<RT, true>, a, grid, grid.x, apply_smem<RT>(true), s);
-  return launch_cluster(lora_apply_kernel<RT, false>, a, grid, grid.x, apply_smem<RT>(false), s);
+  if (large && across) return launch<lora_tile_kernel<RT, true>>(a, grid, tile_smem<RT>(), s);
+  if (large) return launch<lora_tile_kernel<RT, false>>(a, grid, tile_smem<RT>(), s);
+  if (across) return launch<lora_apply_kernel<RT, true>>(a, grid, apply_smem<RT>(true), s);
+  return launch<lora_apply_kernel<RT, false>>(a, grid, apply_smem<RT>(false), s);
 }
 
 inline int bound_tiles(int T, int E, int size) {
@@ -990,11 +978,11 @@ int factor_grad(const GradArgs& a, int E, cudaStream_t s) {
   int c = 1;
   while (c < 8 && static_cast<long long>(tiles) * E * c < 148 * 2 && T / E > c * 4 * kTok) c *= 2;
   const dim3 grid(c, tiles, E);
-  if (r <= 8) return launch_cluster(lora_grad_kernel<1>, a, grid, c, grad_smem<1>(), s);
-  if (r <= 16) return launch_cluster(lora_grad_kernel<2>, a, grid, c, grad_smem<2>(), s);
-  if (r <= 32) return launch_cluster(lora_grad_kernel<4>, a, grid, c, grad_smem<4>(), s);
-  if (r <= 64) return launch_cluster(lora_grad_kernel<8>, a, grid, c, grad_smem<8>(), s);
-  return launch_cluster(lora_grad_kernel<16>, a, grid, c, grad_smem<16>(), s);
+  if (r <= 8) return launch<lora_grad_kernel<1>>(a, grid, grad_smem<1>(), s);
+  if (r <= 16) return launch<lora_grad_kernel<2>>(a, grid, grad_smem<2>(), s);
+  if (r <= 32) return launch<lora_grad_kernel<4>>(a, grid, grad_smem<4>(), s);
+  if (r <= 64) return launch<lora_grad_kernel<8>>(a, grid, grad_smem<8>(), s);
+  return launch<lora_grad_kernel<16>>(a, grid, grad_smem<16>(), s);
 }
 
 }  // namespace

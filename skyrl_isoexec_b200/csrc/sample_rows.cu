@@ -1047,22 +1047,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   place(s, sh, a, r, c, rank, value, nth, lead->ties, list, top, per, kept_mass, table);
 }
 
-int launch(void (*kern)(Args), const Args& args, int rows, int cluster, int smem, bool early, cudaStream_t s) {
-  if (smem > 4 * 1024) IX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = smem;
-  cfg.gridDim = dim3(cluster, rows);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = early && ixh::pdl_enabled() ? 2 : 1;
-  IX_CUDA(cudaLaunchKernelEx(&cfg, kern, args));
-  return 0;
+template <auto Kern>
+int launch(const Args& args, int rows, int cluster, int smem, int most, bool early, cudaStream_t s) {
+  return ixh::launch_cluster<Kern>(args, dim3(cluster, rows), kThreads, cluster, smem, most, early, s);
 }
 
 }  // namespace
@@ -1094,18 +1081,16 @@ IX_API int ix_sample_rows(const void* logits, long long ld, int rows, int V, int
   while (c < kMaxCluster && rows * c * 2 <= 148 * 2 && V > c * 8192) c *= 2;
   const int pieces = static_cast<int>(static_cast<long long>(V) * (dtype == 0 ? 2 : 4) / c / 16 + 2);
   const bool alone = static_cast<long long>(rows) * c <= 148;          // one CTA a multiprocessor
-  const auto fits = [&](int other) { return pieces * 16 <= (alone ? 220 : 106) * 1024 - other; };
-  constexpr int kAnyStatic = 44 * 1024, kFew = kWarps * kAlive * 4, kBf16Static = 20 * 1024;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const auto any = [&](void (*kern)(Args), bool early) {
-    a.cached = fits(kAnyStatic + kFew);
+  constexpr int kAnyStatic = 44 * 1024, kFew = kWarps * kAlive * 4, kBf16Static = 20 * 1024, kAll = 220 * 1024;
+  const auto keep = [&](int other) {
+    a.cached = pieces * 16 <= (alone ? kAll : 106 * 1024) - other;
     a.kept = a.cached ? pieces : 0;
-    return launch(kern, a, rows, c, a.kept * 16 + kFew, early, s);
+    return a.kept * 16;
   };
-  if (dtype == 1) return any(sample_any_kernel<float>, false);
-  a.cached = fits(kBf16Static);
-  a.kept = a.cached ? pieces : 0;
-  const int rc = launch(sample_bf16_kernel, a, rows, c, a.kept * 16, false, s);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == 1) return launch<sample_any_kernel<float>>(a, rows, c, keep(kAnyStatic + kFew) + kFew, kAll - kAnyStatic, false, s);
+  const int rc = launch<sample_bf16_kernel>(a, rows, c, keep(kBf16Static), kAll - kBf16Static, false, s);
+  if (rc) return rc;
   // started while the first one drains: it waits for its marks, and nearly always ends there
-  return rc ? rc : any(sample_any_kernel<__nv_bfloat16>, true);
+  return launch<sample_any_kernel<__nv_bfloat16>>(a, rows, c, keep(kAnyStatic + kFew) + kFew, kAll - kAnyStatic, true, s);
 }

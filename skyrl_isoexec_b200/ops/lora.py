@@ -121,6 +121,25 @@ def _apply(x, base, out, down, up, scale, plan, want_h):
     return h
 
 
+def _backward_cuda(dy, x, A, B, scale, h, plan, base, need_x, need_a, need_b):
+    (T, K), (E, N, r) = x.shape, B.shape
+    if not need_x:
+        base = dx = None
+    else:
+        dx = base if base is not None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    dA = torch.empty_like(A) if need_a else None
+    dB = torch.empty_like(B) if need_b else None
+    g = torch.empty(2, T, r, dtype=x.dtype, device=x.device) if need_a else None
+    _native.check(
+        _native.lib().ix_lora_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _native.ptr(base),
+                                       base.stride(0) if base is not None else 0, _native.ptr(dx), dx.stride(0) if dx is not None else 0,
+                                       A.data_ptr(), B.data_ptr(), scale.data_ptr(), *plan._apply_args, plan._offsets_ptr,
+                                       _native.ptr(h) if need_b else None, _native.ptr(g), _native.ptr(dA), _native.ptr(dB), T, K, N, r, E,
+                                       _native.raw_stream(plan.index)),
+        "ix_lora_backward")
+    return dx, dA, dB
+
+
 def _cpu_h(x, A, scale, plan):
     """s (x A^T) of every token with its own adapter, fp32 [T, r]; zero rows without one."""
     h = torch.zeros(x.shape[0], A.shape[1])
@@ -160,22 +179,10 @@ def _backward(dy, x, A, B, scale, h, plan, base, need_x: bool, need_a: bool, nee
     """(dx, dA, dB); ``base``: the other part of dx, added to in place."""
     dx = dA = dB = None
     if x.is_cuda:
+        if torch.cuda.current_device() == plan.index:
+            return _backward_cuda(dy, x, A, B, scale, h, plan, base, need_x, need_a, need_b)
         with torch.cuda.device(plan.index):
-            (T, K), (E, N, r) = x.shape, B.shape
-            if need_x:
-                dx = base if base is not None else torch.empty(T, K, dtype=x.dtype, device=x.device)
-            dA = torch.empty(E, r, K, dtype=x.dtype, device=x.device) if need_a else None
-            dB = torch.empty(E, N, r, dtype=x.dtype, device=x.device) if need_b else None
-            g = torch.empty(2, T, r, dtype=x.dtype, device=x.device) if need_a else None
-            base = base if need_x else None
-            _native.check(
-                _native.lib().ix_lora_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _native.ptr(base),
-                                               base.stride(0) if base is not None else 0, _native.ptr(dx), dx.stride(0) if dx is not None else 0,
-                                               A.data_ptr(), B.data_ptr(), scale.data_ptr(), *plan._apply_args, plan._offsets_ptr,
-                                               _native.ptr(h) if need_b else None, _native.ptr(g), _native.ptr(dA), _native.ptr(dB), T, K, N, r, E,
-                                               _native.raw_stream(x.get_device())),
-                "ix_lora_backward")
-        return dx, dA, dB
+            return _backward_cuda(dy, x, A, B, scale, h, plan, base, need_x, need_a, need_b)
     g = _cpu_h(dy, B.transpose(1, 2), scale, plan)
     if need_x:
         dx = _cpu_up(g, A.transpose(1, 2), plan)
@@ -200,7 +207,7 @@ class _LoraAdd(torch.autograd.Function):
         out, h = _forward(_rows(y), x2, A2, B2, scale, plan, False, ctx.needs_input_grad[3])
         ctx.save_for_backward(x2, A2, B2, scale, h)
         ctx.plan, ctx.xshape = plan, x.shape
-        return out.view(y.shape)
+        return out if y.dim() == 2 else out.view(y.shape)
 
     @staticmethod
     def backward(ctx, dout):
@@ -208,7 +215,7 @@ class _LoraAdd(torch.autograd.Function):
         x, A, B, scale, h = ctx.saved_tensors
         ny, nx, na, nb = ctx.needs_input_grad[:4]
         dx, dA, dB = _backward(_rows(dout), x, A, B, scale, h, ctx.plan, None, nx, na, nb)
-        return (dout if ny else None), (dx.view(ctx.xshape) if nx else None), dA, dB, None, None
+        return (dout if ny else None), (dx.view(ctx.xshape) if nx and len(ctx.xshape) != 2 else dx), dA, dB, None, None
 
 
 class _LoraLinear(torch.autograd.Function):
@@ -229,7 +236,7 @@ class _LoraLinear(torch.autograd.Function):
         base = F.gemm_nn(dy, w) if nx else None
         dx, dA, dB = _backward(dy, x, A, B, scale, h, ctx.plan, base, nx, na, nb)
         dw = F.gemm_tn(dy, x) if nw else None
-        return (dx.view(ctx.xshape) if nx else None), dw, dA, dB, None, None
+        return (dx.view(ctx.xshape) if nx and len(ctx.xshape) != 2 else dx), dw, dA, dB, None, None
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scale: torch.Tensor, plan: LoraPlan) -> torch.Tensor:
