@@ -16,7 +16,7 @@
 // search ends there is marked and left to the second kernel. fp32 rows and marked ones (sample_any_kernel): 2048 equal
 // steps below the maximum with counts and weights, then the step in question digit by digit.
 //
-// Reading the row is the bound, three times (maximum, histogram, place of the token) of which two come from L2.
+// Reading the row is the bound, for the histogram and for the token's place, the second time from L2 or shared memory.
 #include "bw_common.cuh"
 #include "host_util.h"
 
@@ -215,6 +215,7 @@ __device__ __forceinline__ double two_to_minus(double t, const double* table) {
 struct Shared {                       // of one CTA; rank 0's copy is the cluster's
   float top[kWarps], low[kWarps];
   float cta_top, cta_low;
+  int cta_bad;
   double sd[kWarps];
   u64 su[kWarps];
   unsigned sc[kWarps];
@@ -230,6 +231,31 @@ struct Shared {                       // of one CTA; rank 0's copy is the cluste
   // what place() finds
   unsigned found_n, found_min;
 };
+
+// The threads' largest and smallest values over the cluster; whether any of them says `bad`.
+__device__ __forceinline__ bool over_cluster(float hi, float lo, bool bad, Shared& sh, int c, float& top, float& low) {
+  bad = __any_sync(0xffffffffu, bad);
+  hi = warp_all(hi, [](float a, float b) { return fmaxf(a, b); });
+  lo = warp_all(lo, [](float a, float b) { return fminf(a, b); });
+  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo, sh.sc[threadIdx.x >> 5] = bad;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.top[w]), lo = fminf(lo, sh.low[w]), bad |= sh.sc[w] != 0u;
+  if (c > 1) {
+    if (threadIdx.x == 0) sh.cta_top = hi, sh.cta_low = lo, sh.cta_bad = bad;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q) {
+      if (q < c) {
+        const Shared* o = cl.map_shared_rank(&sh, q);
+        hi = fmaxf(hi, o->cta_top), lo = fminf(lo, o->cta_low), bad |= o->cta_bad != 0;
+      }
+    }
+  }
+  top = hi, low = lo;
+  return bad;
+}
 
 // The row's largest value and its smallest one, over the cluster, without NaN; fills the kept pieces.
 template <typename T>
@@ -251,25 +277,7 @@ __device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, f
       for (int q = 0; q < 4; ++q) hi = fmaxf(hi, x[q]), lo = fminf(lo, x[q]);
     });
   }
-  hi = warp_all(hi, [](float a, float b) { return fmaxf(a, b); });
-  lo = warp_all(lo, [](float a, float b) { return fminf(a, b); });
-  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.top[w]), lo = fminf(lo, sh.low[w]);
-  if (c > 1) {
-    if (threadIdx.x == 0) sh.cta_top = hi, sh.cta_low = lo;
-    cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-#pragma unroll
-    for (int q = 0; q < kMaxCluster; ++q) {
-      if (q < c) {
-        const Shared* o = cl.map_shared_rank(&sh, q);
-        hi = fmaxf(hi, o->cta_top), lo = fminf(lo, o->cta_low);
-      }
-    }
-  }
-  top = hi, low = lo;
+  over_cluster(hi, lo, false, sh, c, top, low);
 }
 
 // Index of the nth (from 0) element that equals `value`, for any number of them: warps own neighbouring pieces, so counts in
@@ -451,53 +459,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
   fill_table(table);
   if (tid == 0) sh.found_n = 0u, sh.found_min = 0xffffffffu;
-  float top, low;
-  extremes(s, sh, c, top, low);
-  cg::cluster_group cl = cg::this_cluster();
-  if (top == -INFINITY || row.greedy) {                 // the same for the whole cluster
-    if (c > 1) cl.sync();                               // peers have read this CTA's extremes
-    if (top == -INFINITY) {
-      if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY, a.marked[r] = 0;
-      return;
-    }
-    if (rank == 0 && tid == 0) a.marked[r] = 0;
-    place(s, sh, a, r, c, rank, top, 0u, 1u, bins, top, 1.0, 1.0, table);
-    return;
-  }
-  low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
-  // magnitudes are compared as integers: `base` is the first one of the lowest binade with bins of its own. What is larger
-  // than the widest one is negative and below the window, or no number; where the widest is infinite the row is marked
-  const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };
-  const int widest = max(mag(top), mag(low)) >> 7;
-  const int base = max(0, (widest - (kBinades - 1)) << 7), first = max(1, base);
+  // The bins are the 16 binades from the widest magnitude of the window down. The row's first 4096 tokens suggest it, with a
+  // binade to spare, so that one pass finds the extremes and counts; where the row then says otherwise, it is counted again.
+  const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };   // compared as integers
   const double per = 1.4426950408889634 / row.T;
-  const auto weigh_value = [&](float x) { return x == top ? 1.0 : two_to_minus((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
-  unsigned zeros = 0, tiny = 0;
-  u64 tiny_mass = 0;
+  int base, first;                    // magnitudes: the lowest binade's first, and the first that has a bin
+  unsigned some;                      // how many have one
+  unsigned *up, *downward;            // bins of distance 0 from `first`, and one past the first negative one (-d is ~d + 1)
+  const auto lay_out = [&](int widest) {
+    base = max(0, (widest - (kBinades - 1)) << 7), first = max(1, base);
+    some = kHalf + base - first;
+    up = bins + kHalf + 1 + (first - base), downward = bins + kHalf - (first - base);
+  };
+  unsigned zeros = 0, tiny = 0;       // tokens that are zero, or closer to it than the bins reach
+  u64 tiny_mass = 0;                  // weight of the latter, relative to the value `ref`, in 2^-44
+  float ref = 0.f;
+  bool above = false;
   const auto around_zero = [&](unsigned bits, unsigned n) {
     if (bits & 0x7fffu) {
       const float x = __uint_as_float(bits << 16);
       tiny += n;
-      if (x >= low) tiny_mass += n * static_cast<u64>(weigh_value(x) * 17592186044416.0 + 0.5);     // 2^44
+      if (x > ref) above = true;
+      else tiny_mass += n * static_cast<u64>(two_to_minus((static_cast<double>(ref) - static_cast<double>(x)) * per, table) * 17592186044416.0 + 0.5);
     } else {
       zeros += n;
     }
   };
-  // distance from the first magnitude with a bin: less than kHalf of them have one, a negative distance is around zero
-  const unsigned some = kHalf + base - first;
-  unsigned* const up = bins + kHalf + 1 + (first - base);
-  unsigned* const downward = bins + kHalf - (first - base);        // one past the first negative bin: -d is ~d + 1
   const auto add = [&](unsigned bits, unsigned n) {
     const int d = static_cast<int>(bits & 0x7fffu) - first;
     const int sign = -static_cast<int>(bits >> 15 & 1u);
     if (static_cast<unsigned>(d) < some) atomicAdd((sign ? downward : up) + (d ^ sign), n);
     return d;
   };
-  s.edges([&](__nv_bfloat16 x) {
-    const unsigned bits = __bfloat16_as_ushort(x);
-    if (add(bits, 1u) < 0) around_zero(bits, 1u);
-  });
-  s.pieces<false>([&](const uint4& w) {
+  const auto count_edges = [&]() {
+    s.edges([&](__nv_bfloat16 x) {
+      const unsigned bits = __bfloat16_as_ushort(x);
+      if (add(bits, 1u) < 0) around_zero(bits, 1u);
+    });
+  };
+  const auto count = [&](const uint4& w) {
     if (w.x == w.y && w.z == w.w && w.x == w.z && (w.x >> 16) == (w.x & 0xffffu)) {          // a mask's run: one atomic, not eight
       if (add(w.x & 0xffffu, 8u) < 0) around_zero(w.x & 0xffffu, 8u);
       return;
@@ -511,7 +511,73 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
         if (static_cast<int>(bits & 0x7fffu) < first) around_zero(bits, 1u);
       }
     }
-  });
+  };
+  float top, low;
+  int guess = -1;
+  bool bad = false;
+  if (!row.greedy && !s.cached) {                       // (a second pass over shared memory is no more than the look ahead)
+    __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY), l = __float2bfloat162_rn(INFINITY);
+    if (tid < (a.V - s.first) / 8) {
+      const uint4 w = s.vec[tid];
+      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h = __hmax2(h, x[q]), l = __hmin2(l, x[q]);
+    }
+    const float hi = warp_all(fmaxf(__low2float(h), __high2float(h)), [](float x, float y) { return fmaxf(x, y); });
+    const float lo = warp_all(fminf(__low2float(l), __high2float(l)), [](float x, float y) { return fminf(x, y); });
+    if ((tid & 31) == 0) sh.top[tid >> 5] = hi, sh.low[tid >> 5] = lo;
+    __syncthreads();                                    // (the bins are zero, too)
+    top = -INFINITY, low = INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.top[w]), low = fminf(low, sh.low[w]);
+    __syncthreads();
+    low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
+    if (top > -INFINITY && top < INFINITY) guess = min(254, (max(mag(top), mag(low)) >> 7) + 1);
+  }
+  if (guess >= 0) {
+    lay_out(guess);
+    ref = top;
+    float hi = -INFINITY, lo = INFINITY;
+    count_edges();
+    s.edges([&](__nv_bfloat16 x) { hi = fmaxf(hi, __bfloat162float(x)), lo = fminf(lo, __bfloat162float(x)); });
+    __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY), l = __float2bfloat162_rn(INFINITY);
+    s.pieces<true>([&](const uint4& w) {
+      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h = __hmax2(h, x[q]), l = __hmin2(l, x[q]);
+      count(w);
+    });
+    hi = fmaxf(hi, fmaxf(__low2float(h), __high2float(h))), lo = fminf(lo, fminf(__low2float(l), __high2float(l)));
+    bad = over_cluster(hi, lo, above, sh, c, top, low);
+  } else {
+    extremes(s, sh, c, top, low);
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  if (top == -INFINITY || row.greedy) {                 // the same for the whole cluster
+    if (c > 1) cl.sync();                               // peers have read this CTA's extremes
+    if (top == -INFINITY) {
+      if (rank == 0 && tid == 0) a.tokens[r] = 0, a.logprobs[r] = -INFINITY, a.marked[r] = 0;
+      return;
+    }
+    if (rank == 0 && tid == 0) a.marked[r] = 0;
+    place(s, sh, a, r, c, rank, top, 0u, 1u, bins, top, 1.0, 1.0, table);
+    return;
+  }
+  low = fmaxf(low, top - kWindow * static_cast<float>(row.T));
+  // What is larger than the widest magnitude is negative and below the window, or no number; where the widest is infinite the
+  // row is marked
+  const int widest = max(mag(top), mag(low)) >> 7;
+  const auto weigh_value = [&](float x) { return x == top ? 1.0 : two_to_minus((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
+  if (guess < 0 || bad || widest > guess || widest + 3 < guess) {
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
+    __syncthreads();
+    zeros = 0, tiny = 0, tiny_mass = 0;
+    lay_out(widest);
+    ref = top;
+    count_edges();
+    s.pieces<false>(count);
+  }
   // what lies around zero, summed over the CTA
   zeros = warp_all(zeros, Add()), tiny = warp_all(tiny, Add()), tiny_mass = warp_all(tiny_mass, Add());
   __shared__ unsigned s_zero[kWarps], s_tiny[kWarps];
@@ -563,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       for (int q = 0; q < kMaxCluster; ++q)
         if (q < c) zc += vz[q], tc += vt[q], tm += vm[q];
     }
-    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) + (zc ? zc * weigh_value(0.f) : 0.0);
+    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) * two_to_minus((static_cast<double>(top) - static_cast<double>(ref)) * per, table) + (zc ? zc * weigh_value(0.f) : 0.0);
     const unsigned mid = zc + tc;
     const int place0 = tid * kEach;
     const bool after_mid = place0 == kHalf;

@@ -118,6 +118,33 @@ def test_shapes_of_the_distribution(dev, dtype):
         _check(x, torch.rand(n, generator=gen), m=m)
 
 
+@pytest.mark.gpu
+def test_rows_whose_beginning_says_nothing_about_the_rest():
+    """Long rows in a large batch are laid out by their first tokens: all kinds of beginnings that mislead."""
+    gen = torch.Generator().manual_seed(11)
+    V, n = 60001, 160
+    x = torch.randn(n, V, generator=gen) * 2
+    x[0:10, :5000] = float("-inf")                                   # nothing there
+    x[10:20, :5000] *= 1e-4                                          # much smaller than the rest
+    x[20:30, :5000] *= 40                                            # and much larger
+    x[30:40] = torch.where(x[30:40] > 7.9, x[30:40], x[30:40] * 1e-6)
+    x[40:50, :5000] = -x[40:50, :5000].abs() - 1                     # all below zero, the rest next to it
+    x[40:50, 5000:] *= 1e-7
+    x[50:60, 55000] = 60.0                                           # the largest comes late
+    x[60:70, :5000] = 0.0
+    x[70:80, :5000] = float("nan")
+    x[80:90, 59999] = float("inf")
+    x[90:100] = -x[90:100].abs() * 30
+    x[90:100, 50000:] = -1e-3
+    x[100:110, 1:] = float("-inf")
+    x[110:120, :4200] = -1e30
+    x[120:130] = -1e-6 * x[120:130].abs()
+    x[120:130, 5000] = 1e-3
+    x = x.bfloat16().cuda()
+    for trial in range(2):
+        _check(x, torch.rand(n, generator=gen), **(_settings(n, gen) if trial else {}))
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masks_infinities_and_nan(dev, dtype):
