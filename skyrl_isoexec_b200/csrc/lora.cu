@@ -746,7 +746,7 @@ constexpr int grad_smem() {
 }
 
 template <int RT>
-__global__ void __launch_bounds__(256) lora_grad_kernel(const __grid_constant__ GradArgs p) {
+__global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_kernel(const __grid_constant__ GradArgs p) {
   extern __shared__ __align__(128) uint8_t raw[];
   const int c = gridDim.x, rank_cta = blockIdx.x, a = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l8 = lane & 7, lm = lane >> 3;
@@ -973,10 +973,16 @@ int factor_grad(const GradArgs& a, int E, cudaStream_t s) {
     IX_CUDA(cudaMemsetAsync(a.out, 0, static_cast<size_t>(E) * r * a.C * 2, s));
     return 0;
   }
-  // CTAs an adapter's columns: until the card has two a multiprocessor, but not beyond four tiles of an average adapter's
-  // tokens each (8192 tokens x 24576: 79 us with 2, 117 with 1, 84 with 4; 463 tokens an adapter: 8 us with 2, 11 with 4)
+  // CTAs an adapter's columns, with at least four tiles of an average adapter's tokens each: what gives the shortest run of
+  // CTAs one after another on a multiprocessor's places, the fewest where that is equal (8192 tokens x 24576: 79 us with 2,
+  // 117 with 1, 84 with 4; 463 tokens an adapter: 8 us with 2, 11 with 4)
+  const long long places = 148 * (r <= 16 ? 3 : r <= 64 ? 2 : 1), all = static_cast<long long>(tiles) * E;
   int c = 1;
-  while (c < 8 && static_cast<long long>(tiles) * E * c < 148 * 2 && T / E > c * 4 * kTok) c *= 2;
+  long long best = (all + places - 1) / places * 8;
+  for (int k = 2; k <= 8 && T / E >= k * 4 * kTok; k *= 2) {
+    const long long turns = (all * k + places - 1) / places * (8 / k);
+    if (turns < best) best = turns, c = k;
+  }
   const dim3 grid(c, tiles, E);
   if (r <= 8) return launch<lora_grad_kernel<1>>(a, grid, grad_smem<1>(), s);
   if (r <= 16) return launch<lora_grad_kernel<2>>(a, grid, grad_smem<2>(), s);
