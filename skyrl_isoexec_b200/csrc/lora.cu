@@ -18,7 +18,7 @@
 // both operands agree, so a lane's 8 neighbours feed two products of depth 16.
 //
 // Measured (6.54 TB/s is a copy): 48 tokens of 32 adapters, 4096 -> 6144, rank 16: 7.3 us, of which 5 are the latency of one
-// token's; 8192 tokens, 4096 -> 24576, rank 16: 163 us, 5.3 TB/s; dx the other way 107 us, 4.4 TB/s; dB 79 us, 5.1 TB/s;
+// token's; 8192 tokens, 4096 -> 24576, rank 16: 163 us, 5.3 TB/s; dx the other way 104 us, 4.5 TB/s; dB 79 us, 5.1 TB/s;
 // 4093 tokens, 4096 -> 4096, rank 64: 34 us, 3.2 TB/s, bound by shared memory and the two products of each h.
 #include "bw_common.cuh"
 #include "host_util.h"
@@ -952,14 +952,14 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   a.n_tiles = static_cast<const int*>(n_tiles) + large;
   const int tiles = bound_tiles(T, E, large ? kLarge : kSmall);
   if (tiles > 65535) return ixh::fail(ixh::IX_ESIZE, "lora: %d tokens of %d adapters make more than 65535 tiles", T, E);
-  // CTAs a tile: as many as run together, but not beyond eight steps (small: one a warp) each; where a large tile's CTA then
-  // still has 96 stages, once more: the last CTAs to run are shorter (8192 x 4096 -> 24576: 189 us with 4, 163 with 8; with 32
-  // stages each, 44 us either way, and rank 64 loses from 66 to 77)
+  // CTAs a tile: as many as run together, but not beyond eight steps (small: one a warp) each. 8192 tokens 4096 -> 4096: 44 us
+  // with 4 at rank 16 (2: 48, 8: 45), 52 with 2 at rank 32 (4: 66), 61 with 2 at rank 64 (4: 66, 1: 75). Where a tile of rank
+  // up to 16 has a long row to write, once more: 4096 -> 24576 takes 163 us with 8, 190 with 4 (ranks 32 and 64 do not gain)
   int c = 1;
   const int widest = (K > N ? K : N) / 32;
   const int together = 148 * (!large || r <= 16 ? 4 : r <= 32 ? 3 : r <= 64 ? 2 : 1);
   while (c < 8 && tiles * c * 2 <= together && widest > c * 8) c *= 2;
-  if (large && c < 8 && (K + N) / 64 >= 96 * c) c *= 2;
+  if (large && r <= 16 && !across && c < 8 && N / 64 >= 64 * c) c *= 2;
   const dim3 grid(c, tiles);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (r <= 8) return apply_tile<1>(a, large, across, grid, s);
