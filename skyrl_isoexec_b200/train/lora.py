@@ -139,7 +139,8 @@ class AdapterBank:
         self.cfgs = [ad.cfg for ad in adapters.values()]
         self.rank = max(-(-c.rank // 8) * 8 for c in self.cfgs)
         dev = model.store.flat.device
-        self.scale = torch.tensor([ad.scale for ad in adapters.values()], dtype=torch.float32, device=dev)
+        self.scales = [ad.scale for ad in adapters.values()]
+        self.scale = torch.tensor(self.scales, dtype=torch.float32, device=dev)
         self.A: dict[str, torch.Tensor] = {}
         self.B: dict[str, torch.Tensor] = {}
         for t in [n for n in views if any(n in ad.A for ad in adapters.values())]:
@@ -150,6 +151,10 @@ class AdapterBank:
             missing = [t for t in ad.A if t not in self.A]
             if missing:
                 raise ValueError(f"AdapterBank: the model has no weight {missing[0]!r} that adapter {name!r} was made for")
+            merged_only = [t for t in ad.A if not t.endswith(DEFAULT_TARGETS)]
+            if merged_only:
+                raise ValueError(f"AdapterBank: adapter {name!r} has factors of {merged_only[0]!r}; beside the projections only "
+                                 f"{', '.join(DEFAULT_TARGETS)} are computed (AdapterStore merges any weight)")
             self.put(name, ad)
         for t in self.parameters():
             t.requires_grad_(trainable)
@@ -158,8 +163,11 @@ class AdapterBank:
     def put(self, name: str, ad: LoRAAdapter) -> None:
         """Take the factors of ``ad`` again (after it stepped on its own) in the place of adapter ``name``."""
         e, r = self.names.index(name), ad.cfg.rank
-        if r > self.rank or ad.scale != float(self.scale[e]):
+        if r > self.rank or ad.scale != self.scales[e]:
             raise ValueError(f"AdapterBank: {name!r} changed its rank or scale; build a new bank")
+        if any(t not in self.A for t in ad.A):
+            raise ValueError(f"AdapterBank: {name!r} has new targets; build a new bank")
+        self.cfgs[e] = ad.cfg                                    # (its rank may be another one, under the same scale)
         for t in self.A:
             self.A[t][e].zero_()
             self.B[t][e].zero_()

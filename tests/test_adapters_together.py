@@ -281,3 +281,20 @@ def test_bank_refusals_and_round_trip():
         bank.put("tenant0", LoRAAdapter.init(model, LoRAConfig(rank=32, alpha=64.0)))
     part = LoRAAdapter.init(model, LoRAConfig(rank=4, targets=("attn.o.weight",)))
     assert set(AdapterBank(model, {"x": part}).A) == {f"layers.{i}.attn.o.weight" for i in range(2)}
+
+
+def test_bank_takes_a_scale_that_fp32_rounds_and_refuses_targets_that_are_only_merged():
+    model = _model("cpu")
+    ad = LoRAAdapter.init(model, LoRAConfig(rank=12, alpha=16.0))
+    bank = AdapterBank(model, {"x": ad})
+    bank.put("x", ad)
+    assert bank.scale.item() == torch.tensor(16 / 12).item()
+    wide = LoRAAdapter.init(model, LoRAConfig(rank=4, targets=("attn.o.weight", "embed.weight")))
+    with pytest.raises(ValueError, match="only .* are computed"):
+        AdapterBank(model, {"x": wide})
+    part = AdapterBank(model, {"x": LoRAAdapter.init(model, LoRAConfig(rank=12, alpha=16.0, targets=("attn.o.weight",)))})
+    with pytest.raises(ValueError, match="new targets"):
+        part.put("x", ad)
+    grown = LoRAAdapter.init(model, LoRAConfig(rank=15, alpha=20.0))
+    bank.put("x", grown)
+    assert all(torch.equal(bank.adapter("x").A[t], grown.A[t].to(bank.A[t].dtype).float()) for t in grown.A)
