@@ -48,6 +48,15 @@ class LoraPlan:
             _native.check(L.ix_lora_plan(ids.data_ptr(), self.T, self.E, self._apply_args[0], self._offsets_ptr, *self._apply_args[1:],
                                          _native.stream()), "ix_lora_plan")
 
+    def record_stream(self, stream) -> None:
+        """As ``torch.Tensor.record_stream`` on the plan's buffers: for a plan that another stream than its own still reads
+        when it is dropped."""
+        if self.device.type == "cuda":
+            self.perm.record_stream(stream)              # (all buffers are one allocation)
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("a LoraPlan is tied to its buffers on the device: build another one from the ids")
+
 
 def pad_rank(A: torch.Tensor, B: torch.Tensor, rank: int) -> tuple[torch.Tensor, torch.Tensor]:
     """One adapter's ``A [r, K]`` and ``B [N, r]`` filled up with zeros to ``rank``."""

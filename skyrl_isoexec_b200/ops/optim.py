@@ -32,7 +32,7 @@ class TensorAdamW:
     Gradients are read from ``grads``, one buffer per parameter that the program fills again for every step (autograd, a
     projection, ``F.gemm_tn(out=...)``); without the argument they are made here, fp32 zeros in one allocation
     (``zero_grad`` clears them). The memory of parameters and gradients is fixed at construction (and kept alive): a step does
-    no per-tensor work on the host, and does not see a ``p.data`` that was replaced.
+    no per-tensor work on the host, and does not see a ``p.data`` or an entry of ``state`` that was replaced.
 
     ``state_bits=8``: both moments in e4m3 with one scale per 256 elements, the second by its square root, 2 bytes and a bit
     per element instead of 8. ``state`` holds flat buffers in which tensor ``i`` starts at ``offsets[i]`` (a multiple of
@@ -88,8 +88,12 @@ class TensorAdamW:
         if dt == torch.bfloat16:
             self.state["master"] = torch.zeros(total, dtype=torch.float32, device=dev)
             self.refresh_masters()
+        self._memory += self.state.values()
         if dev.type == "cuda":
             self._tables()
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("TensorAdamW is tied to the memory of its parameters: build another one and pass state_dict() on")
 
     def _tables(self) -> None:
         chunk = _native.lib().ix_tensor_adamw_chunk()

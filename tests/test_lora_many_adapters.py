@@ -307,3 +307,26 @@ def test_captured_replayed_repeated_and_on_another_stream(T):
         a.copy_(b)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, once()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_plan_is_not_copied_and_may_be_dropped_while_another_stream_reads_it(dev):
+    import copy
+
+    y, x, A, B, scale, ids, _ = _make(4000, 64, 48, 8, 2, "shuffled", dev)
+    plan = LoraPlan(ids, 2)
+    for call in (copy.copy, copy.deepcopy):
+        with pytest.raises(TypeError, match="from the ids"):
+            call(plan)
+    want = lora_add(y, x, A, B, scale, plan)
+    if dev == "cpu":
+        return plan.record_stream(None)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [lora_add(y, x, A, B, scale, plan) for _ in range(20)]
+    plan.record_stream(s)
+    del plan
+    junk = [torch.zeros(60000, dtype=torch.int32, device="cuda") for _ in range(4)]       # (zeros index nothing out of range)
+    torch.cuda.current_stream().wait_stream(s)
+    assert len(junk) == 4 and all(torch.equal(g, want) for g in got)

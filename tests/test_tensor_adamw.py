@@ -160,6 +160,20 @@ def test_replaced_storage_is_neither_stepped_nor_freed(dev):
         assert not w.any() and not any(j.any() for j in junk)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_copies_are_refused_and_replaced_states_stay_allocated(dev):
+    import copy
+
+    w = torch.ones(300, device=dev)
+    opt = TensorAdamW([w], grads=[torch.ones(300, device=dev)], lr=0.1, state_bits=8)
+    for call in (copy.copy, copy.deepcopy):
+        with pytest.raises(TypeError, match="state_dict"):
+            call(opt)
+    old = dict(opt.state)
+    opt.state["exp_avg"] = torch.zeros_like(opt.state["exp_avg"])
+    assert all(any(t is m for m in opt._memory) for t in old.values())
+
+
 @pytest.mark.gpu
 def test_another_stream_capture_refused_and_version_counters():
     torch.manual_seed(2)
