@@ -18,8 +18,9 @@
 //
 // A row is read for the histogram and for the token's place, the second time from L2 or shared memory. Measured: one bf16 row of
 // 151936 17 us, 67 rows of 128256 27 us, which is the latency of their steps; 512 rows of 151936 104 us: a turn of 296 rows
-// takes 52 us, 20 of them reading and counting (a warp's 32 atomics 1.5 to 2 ns), 12 looking for the token, and the rest waiting
-// on sums in 64 bits and on each other. 24 fp32 rows of 248320 with 3 % of the tokens left 48 us, 256 full ones of 151936
+// takes 50 us, 27 of them reading and counting (a warp's 32 atomics 1.5 ns, 14 us in all, beside 14 of reading), 9 looking for
+// the token, and the rest the look ahead, sums in 64 bits and waiting
+// on each other. 24 fp32 rows of 248320 with 3 % of the tokens left 48 us, 256 full ones of 151936
 // 303 us: there every token's weight is computed in 64 bits (6 ns for a warp's).
 #include "bw_common.cuh"
 #include "host_util.h"
