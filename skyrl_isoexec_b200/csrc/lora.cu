@@ -122,10 +122,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ uint4 ld16(const __nv_bfloat16* p, bool ok) {
   return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
 }
-// x = hi + lo, two bf16 numbers; packed pairs
+// x = hi + lo, two bf16 numbers; packed pairs. An infinite number leaves no rest (infinity less infinity is none)
+__device__ __forceinline__ float rest_of(float x, float hi) { return fabsf(hi) < INFINITY ? x - hi : 0.f; }
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
+  const __nv_bfloat162 l = __floats2bfloat162_rn(rest_of(x, __low2float(h)), rest_of(y, __high2float(h)));
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -237,8 +238,9 @@ __global__ void __launch_bounds__(kWarps * 32) lora_apply_kernel(const __grid_co
     float* mine = smem + warp * 16 * LD;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
-      *reinterpret_cast<float2*>(mine + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(mine + r1 * LD + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+      const bool real = RT <= 2 || 8 * j < p.r;        // ranks that only fill up are zero, not 0 times an infinite x
+      *reinterpret_cast<float2*>(mine + r0 * LD + 8 * j + 2 * t) = real ? make_float2(acc[j][0], acc[j][1]) : make_float2(0.f, 0.f);
+      *reinterpret_cast<float2*>(mine + r1 * LD + 8 * j + 2 * t) = real ? make_float2(acc[j][2], acc[j][3]) : make_float2(0.f, 0.f);
     }
   }
   __syncthreads();
@@ -563,8 +565,9 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT <= 4 ? 3 : RT <= 8 ? 2 :
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       const float2 u = *reinterpret_cast<const float2*>(hfin + r0 * LD + 8 * j + 2 * t), v = *reinterpret_cast<const float2*>(hfin + r1 * LD + 8 * j + 2 * t);
-      *reinterpret_cast<float2*>(hsum + r0 * LD + 8 * j + 2 * t) = make_float2(acc[j][0] + u.x, acc[j][1] + u.y);
-      *reinterpret_cast<float2*>(hsum + r1 * LD + 8 * j + 2 * t) = make_float2(acc[j][2] + v.x, acc[j][3] + v.y);
+      const bool real = RT <= 2 || 8 * j < p.r;        // ranks that only fill up are zero, not 0 times an infinite x
+      *reinterpret_cast<float2*>(hsum + r0 * LD + 8 * j + 2 * t) = real ? make_float2(acc[j][0] + u.x, acc[j][1] + u.y) : make_float2(0.f, 0.f);
+      *reinterpret_cast<float2*>(hsum + r1 * LD + 8 * j + 2 * t) = real ? make_float2(acc[j][2] + v.x, acc[j][3] + v.y) : make_float2(0.f, 0.f);
     }
   }
   const float sc = p.scale[tile.x];
@@ -727,6 +730,8 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 4 : RT <= 4 ? 3 : RT <= 8 ? 2 :
 // shared memory) from tiles of 64 tokens that asynchronous copies bring in kStages deep; a thread looks up the rows it
 // copies one tile ahead. Warp (w, f) owns 32 columns, all ranks and one half of a tile's tokens. h is the two bf16 numbers
 // that the kernels above stored; sums are fp32, those of the halves and of the cluster are added in order.
+// An infinite z times h's two parts, whose signs may differ, is no number where z h is infinite. So a cluster that finds one
+// among its results sums the first parts alone once more and takes those sums there.
 struct GradArgs {
   const __nv_bfloat16* h;     // [2, T, r], plan's order
   const __nv_bfloat16* z;     // [T, C] rows by token
@@ -747,12 +752,15 @@ constexpr int grad_stage() {
 template <int RT>
 constexpr int grad_smem() {
   const int ring = kStages * grad_stage<RT>(), sums = kCols * (8 * RT + 4) * 4;
-  return ring > sums ? ring : sums;
+  return (ring > sums ? ring : sums) + 16;             // and the word of grad_sums
 }
 
-template <int RT>
-__global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_kernel(const __grid_constant__ GradArgs p) {
+// BOTH: both parts of h, or the first alone for the results that were no numbers. A word behind the ring, set in every CTA of
+// the cluster, says that there are such.
+template <int RT, bool BOTH>
+__device__ __forceinline__ void grad_sums(const GradArgs& p) {
   extern __shared__ __align__(128) uint8_t raw[];
+  int* again = reinterpret_cast<int*>(raw + grad_smem<RT>() - 16);
   const int c = gridDim.x, rank_cta = blockIdx.x, a = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l8 = lane & 7, lm = lane >> 3;
   const int cg4 = warp & 3, hf = warp >> 2;
@@ -826,7 +834,7 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) ldsm4t(hs + (lm >> 1) * kTok * 16 * RT + narrow_at<RT>(k + l8 + 8 * (lm & 1), j0 + j), b[j]);
 #pragma unroll
-        for (int u = 0; u < 4; u += 2)
+        for (int u = 0; u < (BOTH ? 4 : 2); u += 2)
 #pragma unroll
           for (int j = 0; j < kGroup; ++j)
 #pragma unroll
@@ -872,6 +880,14 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_
     for (int k = 0; k < 8; ++k)
       if (k < c) v.x += w[k].x, v.y += w[k].y, v.z += w[k].z, v.w += w[k].w;
     if (col0 + col < p.C && q < p.r) {
+      if constexpr (!BOTH) {                           // only what was no number is taken
+        const __nv_bfloat16* had = p.by_cols ? out + static_cast<size_t>(col0 + col) * p.r + q : out + static_cast<size_t>(q) * p.C + col0 + col;
+        const size_t step = p.by_cols ? 1 : p.C;
+        const float x = __bfloat162float(had[0]), y = __bfloat162float(had[step]), z = __bfloat162float(had[2 * step]), u = __bfloat162float(had[3 * step]);
+        v = make_float4(x == x ? x : v.x, y == y ? y : v.y, z == z ? z : v.z, u == u ? u : v.w);
+      } else if (v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w) {
+        for (int k = 0; k < c; ++k) *cl.map_shared_rank(again, k) = 1;
+      }
       const __nv_bfloat162 lo2 = __floats2bfloat162_rn(v.x, v.y), hi2 = __floats2bfloat162_rn(v.z, v.w);
       if (p.by_cols) {
         uint2 both;
@@ -883,7 +899,20 @@ __global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_
       }
     }
   }
-  cl.sync();
+  cl.sync();                                           // nobody reads a peer's sums after this, and all know of the results
+}
+template <int RT>
+__device__ __noinline__ void grad_sums_of_first_parts(const GradArgs& p) {
+  grad_sums<RT, false>(p);
+}
+
+template <int RT>
+__global__ void __launch_bounds__(256, RT <= 2 ? 3 : RT <= 8 ? 2 : 1) lora_grad_kernel(const __grid_constant__ GradArgs p) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  int* again = reinterpret_cast<int*>(raw + grad_smem<RT>() - 16);
+  if (threadIdx.x == 0) *again = 0;                   // (the cluster's barrier in front of the sums stands between this and the first to set it)
+  grad_sums<RT, true>(p);
+  if (*again) grad_sums_of_first_parts<RT>(p);      // (out of line: the registers are the first sweep's)
 }
 
 // ------------------------------------------------------------------------------------------------ launches

@@ -250,7 +250,9 @@ class _LoraLinear(torch.autograd.Function):
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scale: torch.Tensor, plan: LoraPlan) -> torch.Tensor:
     """``y + s_a (x A_a^T) B_a^T`` for every token's own adapter: x [..., K], y [..., N], A [E, r, K], B [E, N, r], scale [E].
-    One rounding, of the result; a token without an adapter gets y's bits. Differentiable in y, x, A and B."""
+    One rounding, of the result; a token without an adapter gets y's bits. Differentiable in y, x, A and B. An infinite x, A or
+    gradient does what the formula says. An infinite number in the factor of the second product (B; A in the gradient of x) makes
+    infinity or NaN on a GPU: x A^T enters there as the sum of two numbers, whose signs may differ."""
     _check(y, x, A, B, scale, plan)
     scale = _flat(scale)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or y.requires_grad):
