@@ -220,7 +220,6 @@ __device__ __forceinline__ double two_to_minus(double t, const double* table) {
 struct Shared {                       // of one CTA; rank 0's copy is the cluster's
   float top[kWarps], low[kWarps];
   float cta_top, cta_low;
-  int cta_bad;
   double sd[kWarps];
   u64 su[kWarps];
   unsigned sc[kWarps];
@@ -237,29 +236,27 @@ struct Shared {                       // of one CTA; rank 0's copy is the cluste
   unsigned found_n, found_min;
 };
 
-// The threads' largest and smallest values over the cluster; whether any of them says `bad`.
-__device__ __forceinline__ bool over_cluster(float hi, float lo, bool bad, Shared& sh, int c, float& top, float& low) {
-  bad = __any_sync(0xffffffffu, bad);
+// The threads' largest and smallest values over the cluster.
+__device__ __forceinline__ void over_cluster(float hi, float lo, Shared& sh, int c, float& top, float& low) {
   hi = warp_all(hi, [](float a, float b) { return fmaxf(a, b); });
   lo = warp_all(lo, [](float a, float b) { return fminf(a, b); });
-  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo, sh.sc[threadIdx.x >> 5] = bad;
+  if ((threadIdx.x & 31) == 0) sh.top[threadIdx.x >> 5] = hi, sh.low[threadIdx.x >> 5] = lo;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.top[w]), lo = fminf(lo, sh.low[w]), bad |= sh.sc[w] != 0u;
+  for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.top[w]), lo = fminf(lo, sh.low[w]);
   if (c > 1) {
-    if (threadIdx.x == 0) sh.cta_top = hi, sh.cta_low = lo, sh.cta_bad = bad;
+    if (threadIdx.x == 0) sh.cta_top = hi, sh.cta_low = lo;
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
 #pragma unroll
     for (int q = 0; q < kMaxCluster; ++q) {
       if (q < c) {
         const Shared* o = cl.map_shared_rank(&sh, q);
-        hi = fmaxf(hi, o->cta_top), lo = fminf(lo, o->cta_low), bad |= o->cta_bad != 0;
+        hi = fmaxf(hi, o->cta_top), lo = fminf(lo, o->cta_low);
       }
     }
   }
   top = hi, low = lo;
-  return bad;
 }
 
 // The row's largest value and its smallest one, over the cluster, without NaN; fills the kept pieces.
@@ -282,7 +279,7 @@ __device__ __forceinline__ void extremes(const Share<T>& s, Shared& sh, int c, f
       for (int q = 0; q < 4; ++q) hi = fmaxf(hi, x[q]), lo = fminf(lo, x[q]);
     });
   }
-  over_cluster(hi, lo, false, sh, c, top, low);
+  over_cluster(hi, lo, sh, c, top, low);
 }
 
 // Index of the nth (from 0) element that equals `value`, for any number of them: warps own neighbouring pieces, so counts in
@@ -449,7 +446,8 @@ __device__ __forceinline__ void place(const Share<T>& s, Shared& sh, const Args&
 }
 
 // ------------------------------------------------------------------------------------------------ bf16
-constexpr int kBinades = 16, kHalf = kBinades * 128, kBins = 2 * kHalf + 1;   // negative values | around zero | positive ones
+constexpr int kBinades = 16, kHalf = kBinades * 128;                           // what a row is searched in
+constexpr int kRoom = (kBinades + 1) * 128, kBins = 2 * kRoom + 1;             // negative values | around zero | positive ones
 constexpr int kEach = 2 * kHalf / kThreads;                                    // bins a thread searches
 static_assert(kEach * kThreads == 2 * kHalf, "bins are shared out evenly; the middle one goes to a thread of its own place");
 
@@ -464,28 +462,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
   fill_table(table);
   if (tid == 0) sh.found_n = 0u, sh.found_min = 0xffffffffu;
-  // The bins are the 16 binades from the widest magnitude of the window down. The row's first 4096 tokens suggest it, with a
-  // binade to spare, so that one pass finds the extremes and counts; where the row then says otherwise, it is counted again.
+  // The bins are the 16 binades from the widest magnitude of the window down: a function of the row, so that its sums are. A
+  // row's first 4096 tokens suggest them, and one pass finds the extremes and counts, in a binade more, of which either
+  // end may be the one too many; where the row then says otherwise, it is counted again.
   const auto mag = [](float x) { return static_cast<int>((__float_as_uint(x) >> 16) & 0x7fffu); };   // compared as integers
   const double per = 1.4426950408889634 / row.T;
   int base, first;                    // magnitudes: the lowest binade's first, and the first that has a bin
   unsigned some;                      // how many have one
   unsigned *up, *downward;            // bins of distance 0 from `first`, and one past the first negative one (-d is ~d + 1)
-  const auto lay_out = [&](int widest) {
-    base = max(0, (widest - (kBinades - 1)) << 7), first = max(1, base);
-    some = kHalf + base - first;
-    up = bins + kHalf + 1 + (first - base), downward = bins + kHalf - (first - base);
+  const auto lay_out = [&](int widest, int binades) {
+    base = max(0, (widest - (binades - 1)) << 7), first = max(1, base);
+    some = binades * 128 + base - first;
+    up = bins + kRoom + 1 + (first - base), downward = bins + kRoom - (first - base);
   };
   unsigned zeros = 0, tiny = 0;       // tokens that are zero, or closer to it than the bins reach
-  u64 tiny_mass = 0;                  // weight of the latter, relative to the value `ref`, in 2^-44
-  float ref = 0.f;
-  bool above = false;
+  u64 tiny_mass = 0;                  // weight of the latter, relative to that of a zero, in 2^-44
   const auto around_zero = [&](unsigned bits, unsigned n) {
     if (bits & 0x7fffu) {
-      const float x = __uint_as_float(bits << 16);
+      // where zero is in the window, T is at least a 42nd of the widest magnitude, and this is next to 1; elsewhere it counts for nothing
+      const double t = static_cast<double>(__uint_as_float(bits << 16)) * -per;
       tiny += n;
-      if (x > ref) above = true;
-      else tiny_mass += n * static_cast<u64>(two_to_minus((static_cast<double>(ref) - static_cast<double>(x)) * per, table) * 17592186044416.0 + 0.5);
+      if (fabs(t) < 1.0 / 64.0) tiny_mass += n * static_cast<u64>(two_to_minus(t, table) * 17592186044416.0 + 0.5);
     } else {
       zeros += n;
     }
@@ -519,7 +516,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   };
   float top, low;
   int guess = -1;
-  bool bad = false;
   if (!row.greedy && !s.cached) {                       // (a second pass over shared memory is no more than the look ahead)
     __nv_bfloat162 h = __float2bfloat162_rn(-INFINITY), l = __float2bfloat162_rn(INFINITY);
     if (tid < (a.V - s.first) / 8) {
@@ -540,8 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     if (top > -INFINITY && top < INFINITY) guess = min(254, (max(mag(top), mag(low)) >> 7) + 1);
   }
   if (guess >= 0) {
-    lay_out(guess);
-    ref = top;
+    lay_out(guess, kBinades + 1);
     float hi = -INFINITY, lo = INFINITY;
     count_edges();
     s.edges([&](__nv_bfloat16 x) { hi = fmaxf(hi, __bfloat162float(x)), lo = fminf(lo, __bfloat162float(x)); });
@@ -553,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       count(w);
     });
     hi = fmaxf(hi, fmaxf(__low2float(h), __high2float(h))), lo = fminf(lo, fminf(__low2float(l), __high2float(l)));
-    bad = over_cluster(hi, lo, above, sh, c, top, low);
+    over_cluster(hi, lo, sh, c, top, low);
   } else {
     extremes(s, sh, c, top, low);
   }
@@ -573,13 +568,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
   // row is marked
   const int widest = max(mag(top), mag(low)) >> 7;
   const auto weigh_value = [&](float x) { return x == top ? 1.0 : two_to_minus((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
-  if (guess < 0 || bad || widest > guess || widest + 3 < guess) {
+  int shift = 0;                                        // magnitudes with bins below the lowest of the 16 binades
+  if (widest == guess || widest + 1 == guess) {
+    const int low_base = base;
+    base = max(0, (widest - (kBinades - 1)) << 7), shift = base - low_base;
+    const int i = tid & 127;                            // their tokens belong to what is around zero
+    if (tid < 256 && i < shift) {
+      const unsigned bits = static_cast<unsigned>(low_base + i) | (tid >> 7) << 15, n = bins[tid >> 7 ? kRoom - 1 - i : kRoom + 1 + i];
+      if (n) around_zero(bits, n);
+    }
+  } else {
     __syncthreads();
     for (int i = tid; i < kBins; i += kThreads) bins[i] = 0u;
     __syncthreads();
     zeros = 0, tiny = 0, tiny_mass = 0;
-    lay_out(widest);
-    ref = top;
+    lay_out(widest, kBinades);
     count_edges();
     s.pieces<false>(count);
   }
@@ -598,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
     cl.sync();
     // each CTA adds up its share of the bins and puts it into rank 0's
     unsigned* lead_bins = cl.map_shared_rank(bins, 0);
-    for (int i = kBins * rank / c + tid; i < kBins * (rank + 1) / c; i += kThreads) {
+    const int from = kRoom - kHalf - shift, all = 2 * (kHalf + shift) + 1;
+    for (int i = from + all * rank / c + tid; i < from + all * (rank + 1) / c; i += kThreads) {
       unsigned v[kMaxCluster], sum = 0;
 #pragma unroll
       for (int q = 0; q < kMaxCluster; ++q)
@@ -634,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
       for (int q = 0; q < kMaxCluster; ++q)
         if (q < c) zc += vz[q], tc += vt[q], tm += vm[q];
     }
-    const double mid_mass = static_cast<double>(tm) * (1.0 / 17592186044416.0) * two_to_minus((static_cast<double>(top) - static_cast<double>(ref)) * per, table) + (zc ? zc * weigh_value(0.f) : 0.0);
     const unsigned mid = zc + tc;
+    const double mid_mass = mid ? (static_cast<double>(tm) * (1.0 / 17592186044416.0) + zc) * two_to_minus(static_cast<double>(top) * per, table) : 0.0;
     const int place0 = tid * kEach;
     const bool after_mid = place0 == kHalf;
     const auto value_at = [&](int j) {
@@ -648,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int at = place0 + j;
-      n[j] = bins[at < kHalf ? 2 * kHalf - at : 2 * kHalf - 1 - at];
+      n[j] = bins[at < kHalf ? kRoom + shift + kHalf - at : kRoom - shift + kHalf - 1 - at];
       any |= n[j];
     }
     // the thread's values are equally spaced (a binade has 128), so their weights are a geometric series

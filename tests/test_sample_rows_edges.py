@@ -1,0 +1,51 @@
+"""One token per row from one given number (ops/sampling.sample_rows): a row's bits are its own, whatever batch it stands in;
+weights that are small beside the largest; an infinite temperature."""
+import pytest
+import torch
+from test_sample_rows import DEVICES, _settings
+
+from skyrl_isoexec_b200.ops.sampling import sample_rows
+
+
+def _rows(V, gen):
+    """Rows of every kind, and some whose beginning misleads whoever lays a histogram out by it."""
+    z = torch.randn(24, V, generator=gen) * 2
+    x = [z[0], z[1] * 8, z[2] * 0.01, z[3].round(), torch.where(z[4] > 3, 30.0, z[4] * 1e-4), torch.zeros(V), torch.full((V,), -1e-6),
+         torch.where(z[5] > 2, z[5], float("-inf")), -z[6].abs() * 30, z[7] + 500, z[8] * 1e-30, torch.where(z[9] > 0, 1e-4, -1e-4)]
+    small = torch.full((V,), 1.25 * 2.0 ** -11)              # one large number, all others next to zero
+    small[0] = 30.0
+    x += [small, small - 15.0, torch.where(torch.arange(V) == 40000 % V, 60.0, z[10])]
+    for k, factor in ((11, 1e-4), (12, 40.0), (13, 0.0), (14, 2.5), (15, 0.4), (16, 6.0)):
+        row = z[k].clone()
+        row[:5000] *= factor
+        x.append(row)
+    row = z[17].clone()
+    row[:5000], row[20000:] = float("-inf"), row[20000:] * 1e-5
+    x.append(row)
+    for scale in (3.0, 1.0, 0.3):                            # every binade between the largest and far below it has its tokens
+        x.append(torch.where(z[18] > 0, 1.0, -1.0) * scale * 2.0 ** (-24 * torch.rand(V, generator=gen)))
+    return torch.stack(x)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9001, pytest.param(60001, marks=pytest.mark.gpu), pytest.param(151936, marks=pytest.mark.gpu)])
+def test_a_row_has_the_same_bits_in_every_batch(dev, dtype, V):
+    if dev == "cpu" and V > 10000:
+        pytest.skip("no other path there")
+    gen = torch.Generator().manual_seed(V)
+    x = _rows(V, gen).to(dtype).to(dev)
+    n = x.shape[0]
+    big = 300 if dev == "cuda" else 40
+    for trial in range(4):
+        s = _settings(n, gen) if trial else dict(T=torch.ones(n), k=torch.zeros(n, dtype=torch.int64), p=torch.ones(n), m=torch.zeros(n))
+        s = {k: v.to(torch.int32 if k == "k" else torch.float32).to(dev) for k, v in s.items()}
+        u = torch.rand(n, generator=gen).to(dev) if trial > 1 else torch.full((n,), trial * (1 - 2.0 ** -24), device=dev)
+        alone = [sample_rows(x[i:i + 1], u[i:i + 1], *(s[k][i:i + 1] for k in "Tkpm")) for i in range(n)]
+        tokens, lps = (torch.cat(t) for t in zip(*alone))
+        at = torch.arange(big, device=dev) % n
+        many = sample_rows(x[at], u[at], *(s[k][at] for k in "Tkpm"))
+        some = sample_rows(x, u, *(s[k] for k in "Tkpm"))
+        for got in ((many[0], many[1], at), (*some, torch.arange(n, device=dev))):
+            wrong = (got[0] != tokens[got[2]]) | (got[1] != lps[got[2]])
+            assert not wrong.any(), (trial, wrong.nonzero()[:, 0].tolist(), got[1][wrong].tolist(), lps[got[2]][wrong].tolist())
