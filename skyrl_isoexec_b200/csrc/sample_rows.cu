@@ -6,10 +6,11 @@
 // index first. The log-probability is that of the kept, renormalised distribution.
 //
 // No row is sorted. A token's weight depends on its value alone, so everything above is a search in the histogram of the
-// row's values: counts per value, weights per value in 64 bits, prefix sums over values. That keeps the sums over a whole
-// vocabulary exact to 2^-50, which a sum of 150,000 weights rounded to 32 bits is not: u falls next to a border of two
-// tokens often enough to be seen. Only values within kWindow T of the maximum count: what lies below weighs less than
-// 2^-42 of the row together, 2^-18 of the distance between two neighbouring numbers u.
+// row's values: counts per value, weights per value in 64 bits, prefix sums over values. Where 150,000 weights are summed in
+// 32 bits, u falls on the wrong side of a border of two tokens often enough to be seen; here a bf16 row's sums are good to
+// 2^-45 of themselves (what the weights' series is), an fp32 row's to 2^-34 of the largest weight and 2^-45 of themselves.
+// Only values within kWindow T of the maximum count: what lies below weighs less than 2^-41 of the row together, 2^-17 of
+// the distance between two neighbouring numbers u.
 //
 // bf16 rows (sample_bf16_kernel): 16 binades of values below the largest magnitude are 4096 counters in shared memory, one
 // atomic a token. Values closer to zero (a thousandth of a row) share one more, whose weight is summed apart; a row whose
@@ -205,7 +206,8 @@ struct Row {                          // what a row asks for
 __device__ __forceinline__ double weight(float x, float top, double T) { return x == top ? 1.0 : exp((static_cast<double>(x) - static_cast<double>(top)) / T); }
 
 // 2^-t for t >= 0: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven implementation of the
-// exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits, good to 1e-14
+// exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits, good to 2e-14 (t itself is
+// rounded to 2^-47)
 __device__ __forceinline__ void fill_table(double* table) {
   if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x * (-1.0 / 64.0));
 }
@@ -796,7 +798,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_bf16_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------ any type
 constexpr int kSteps = 2048, kStepsEach = kSteps / kThreads;
-constexpr double kUnit = 17592186044416.0;            // 2^44 units of weight: 2^19 tokens of weight 1 fit into 64 bits
+// A row's weights are whole numbers of 2^-44 of the largest, so 2^19 tokens fit into 64 bits. A step's are counted in units
+// smaller by its own power of two (2^-44 of the weight at its beginning, give or take a factor of 2) and rounded once, as
+// their sum: many tokens far below the largest keep their weight.
+constexpr double kUnit = 17592186044416.0;
+__device__ __forceinline__ u64 to_row_units(u64 q, int e) { return e ? (q + (1ull << (e - 1))) >> e : q; }
 
 __device__ __forceinline__ unsigned order_key(float x) {
   const unsigned b = __float_as_uint(x + 0.f);         // -0 is 0
@@ -812,9 +818,10 @@ struct Step {                         // what rank 0 tells the cluster
 };
 constexpr int kList = 1024;
 constexpr int kAlive = 512;           // a warp's places for tokens in the window
-// Whether a search ends in the n tokens that stand behind cc others (weights in units: mm before them, next behind them).
-// 0: the end-th token. 1: the last that begin in front of the aim and among the first `end`. 2: the last that begin at or
-// in front of it. Exactly one of a row's bins, or of a bin's values, says yes: the sums are whole numbers.
+// Whether a search ends in the n tokens that stand behind cc others (weights in the row's units: mm before them, next behind
+// them). 0: the end-th token. 1: the last that begin in front of the aim and among the first `end`. 2: the last that begin at
+// or in front of it. Exactly one of a row's bins, or of a bin's values, says yes: the sums are whole numbers, a bin's in smaller
+// units until they are rounded, which never falls as the sum grows and ends where the bin ends.
 __device__ __forceinline__ bool here(int what, unsigned cc, unsigned n, u64 mm, u64 next, double aim, unsigned end) {
   if (what == 0) return cc < end && end <= cc + n;
   if (what == 1) return (cc == 0 || static_cast<double>(mm) < aim) && cc < end && (!(static_cast<double>(next) < aim) || cc + n >= end);
@@ -872,17 +879,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     return q < static_cast<float>(kSteps - 1) ? static_cast<int>(q) : q >= static_cast<float>(kSteps - 1) ? kSteps - 1 : 0;
   };
   const double per = 1.4426950408889634 / row.T;
-  const auto units = [&](float x) { return x == top ? static_cast<u64>(kUnit) : units_of((static_cast<double>(top) - static_cast<double>(x)) * per, table); };
+  // a step's power of two: the binary logarithm of the weight at its beginning, a little less so that rounded steps keep below it
+  const float fall = inv > 0.f ? static_cast<float>(per / inv * 0.9999) : 0.f;
+  // (60 is 42 log2(e); where T is next to the logits' own rounding, top - low is rounded to more than 42 T)
+  const auto power_of = [&](int bin) { return min(60, static_cast<int>(bin * fall)); };
+  const auto units = [&](float x, int e) { return x == top ? static_cast<u64>(kUnit) : units_of((static_cast<double>(top) - static_cast<double>(x)) * per - e, table); };
   const double floor_units = row.min_p * kUnit;
   unsigned some = 0;
   const auto count_in = [&](float x) {
-    const u64 q = units(x);
-    const int b = bin_of(x);
+    const int b = bin_of(x), e = power_of(b);
+    const u64 q = units(x, e);
     atomicAdd(&cnt[b], 1u);
     add_units(&low_half[b], &high_half[b], q);
     // on the border itself (a unit is 2^-44) the weight decides
-    if (row.min_p > 0.0) some += fabs(static_cast<double>(q) - floor_units) > 2.0 ? static_cast<double>(q) > floor_units : weight(x, top, row.T) >= row.min_p;
-    else ++some;
+    if (row.min_p > 0.0) {
+      const double edge = floor_units * static_cast<double>(1ull << e);
+      some += fabs(static_cast<double>(q) - edge) > 2.0 ? static_cast<double>(q) > edge : weight(x, top, row.T) >= row.min_p;
+    } else {
+      ++some;
+    }
   };
   // A warp gathers what lies in the window and counts it in full groups of 32: a masked row's work in 64 bits is that of the
   // tokens its mask leaves. Where all of them fit, the searches look at these instead of at the row again.
@@ -975,7 +990,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
   if (rank == 0) {
 #pragma unroll
     for (int j = 0; j < kStepsEach; ++j) {
-      n[j] = cnt[tid * kStepsEach + j], m[j] = (static_cast<u64>(high_half[tid * kStepsEach + j]) << 32) + low_half[tid * kStepsEach + j];
+      const int b = tid * kStepsEach + j;
+      n[j] = cnt[b], m[j] = to_row_units((static_cast<u64>(high_half[b]) << 32) + low_half[b], power_of(b));
       count += n[j], mass += m[j];
     }
     unsigned fine = 0;
@@ -1019,7 +1035,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
     const Step first = *cl.map_shared_rank(&step[what][0], 0);
     if (!first.go) continue;
     unsigned prefix = 0, seen = 0;
-    u64 weighed = 0;
+    u64 weighed = 0, inside = 0;                       // what stands in front of the bin in the row's units, and behind that in the bin's
+    const int power = power_of(first.bin);
     if (rank == 0) seen = sh.c0, weighed = sh.su[0];
     if (first.few) {
       // the bin's tokens in a list of rank 0; each finds what stands in front of it by looking at all the others
@@ -1031,12 +1048,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
       cl.sync();
       if (rank == 0) {
         const unsigned many = list_n;
-        for (unsigned i = tid; i < many; i += kThreads) list_units[i] = units(key_value(list[i]));
+        for (unsigned i = tid; i < many; i += kThreads) list_units[i] = units(key_value(list[i]), power);
         __syncthreads();
         for (unsigned i = tid; i < many; i += kThreads) {
           const unsigned k = list[i];
           unsigned dc = seen, dn = 0u;
-          u64 dw = weighed;
+          u64 dw = 0;
           const u64 q = list_units[i];
 #pragma unroll 4
           for (unsigned j = 0; j < many; ++j) {
@@ -1045,10 +1062,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
             if (o > k) ++dc, dw += oq;
             dn += o == k;
           }
-          if (here(what, dc, dn, dw, dw + dn * q, aim, what == 2 ? last : keep)) sh.i0 = k, sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
+          if (here(what, dc, dn, weighed + to_row_units(dw, power), weighed + to_row_units(dw + dn * q, power), aim, what == 2 ? last : keep))
+            sh.i0 = k, sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
         }
         __syncthreads();
-        prefix = sh.i0, seen = sh.c0, weighed = sh.cta_mass;
+        prefix = sh.i0, seen = sh.c0, inside = sh.cta_mass;
       }
     }
     for (int level = 0; level < 4 && !first.few; ++level) {
@@ -1060,7 +1078,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         const unsigned k = order_key(x);
         if (level > 0 && (k >> (shift + 8)) != prefix) return;
         atomicAdd(&dcnt[(k >> shift) & 255u], 1u);
-        add_units(&dlow[(k >> shift) & 255u], &dhigh[(k >> shift) & 255u], units(x));
+        add_units(&dlow[(k >> shift) & 255u], &dhigh[(k >> shift) & 255u], units(x, power));
       });
       cl.sync();
       if (rank == 0) {
@@ -1078,23 +1096,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_any_kernel(const __grid_co
         }
         dc = dn, dw = dm;
         block_prefix(dc, dw, sh.sc, sh.su, da, db);
-        dc += seen, dw += weighed;
+        dc += seen, dw += inside;
         if (dn) {
-          if (here(what, dc, dn, dw, dw + dm, aim, what == 2 ? last : keep)) {
+          if (here(what, dc, dn, weighed + to_row_units(dw, power), weighed + to_row_units(dw + dm, power), aim, what == 2 ? last : keep)) {
             step[what][level + 1].prefix = (prefix << 8) | static_cast<unsigned>(255 - tid);
             sh.c0 = dc, sh.c1 = dn, sh.cta_mass = dw;
           }
         }
         __syncthreads();
-        seen = sh.c0, weighed = sh.cta_mass;
+        seen = sh.c0, inside = sh.cta_mass;
       }
       cl.sync();
       prefix = cl.map_shared_rank(&step[what][level + 1], 0)->prefix;
     }
     if (rank == 0) {
-      // all tokens of one value: seen and weighed stand before them, sh.c1 is their number
+      // all tokens of one value: seen, weighed and inside stand before them, sh.c1 is their number
       const float x = key_value(prefix);
-      const double w = weight(x, top, row.T) * kUnit, front = static_cast<double>(weighed);
+      const double w = weight(x, top, row.T) * kUnit, front = static_cast<double>(weighed) + static_cast<double>(inside) / static_cast<double>(1ull << power);
       const unsigned have = min(sh.c1, (what == 2 ? last : keep) - seen);
       if (what == 0) {
         total = front + (keep - seen) * w;

@@ -1,8 +1,10 @@
 """One token per row from one given number (ops/sampling.sample_rows): a row's bits are its own, whatever batch it stands in;
 weights that are small beside the largest; an infinite temperature."""
+import math
+
 import pytest
 import torch
-from test_sample_rows import DEVICES, _settings
+from test_sample_rows import DEVICES, _check, _settings
 
 from skyrl_isoexec_b200.ops.sampling import sample_rows
 
@@ -49,3 +51,40 @@ def test_a_row_has_the_same_bits_in_every_batch(dev, dtype, V):
         for got in ((many[0], many[1], at), (*some, torch.arange(n, device=dev))):
             wrong = (got[0] != tokens[got[2]]) | (got[1] != lps[got[2]])
             assert not wrong.any(), (trial, wrong.nonzero()[:, 0].tolist(), got[1][wrong].tolist(), lps[got[2]][wrong].tolist())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [4001, pytest.param(524288, marks=pytest.mark.gpu)])
+def test_many_weights_that_are_small_beside_the_largest(dev, dtype, V):
+    """One likely token, all others together some 1e-8 of it: each of them is below any whole number of 2^-44 of the largest."""
+    if dev == "cpu" and V > 100000:
+        pytest.skip("the CPU form sums in 64-bit floating point")
+    rows = []
+    for top, below in ((0.0, 31.21), (30.0, 31.2), (31.2, 31.2), (2.0, 30.0), (1.0, 36.0), (-3.0, 31.2)):
+        row = torch.full((V,), top - below)
+        row[::3] += 0.11
+        row[17] = top
+        rows.append(row)
+    x = torch.stack(rows).to(dtype).to(dev)
+    n = len(rows)
+    u = torch.zeros(n)
+    u[::2] = 1 - 2.0 ** -24
+    _check(x, u)
+    _check(x, u, p=1 - 2.0 ** -24)
+    _check(x, u, T=0.5, m=1e-30)
+    tokens, lps = _check(x[:, :V - 1], u)
+    many = sample_rows(x[:, :V - 1].repeat(30, 1), u.repeat(30).to(dev))
+    assert torch.equal(many[0], tokens.repeat(30)) and torch.equal(many[1], lps.repeat(30))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("at", [0.0, 1000.0, -1000.0, 1e30])
+def test_temperatures_next_to_the_logits_own_rounding(dev, at):
+    """42 temperatures below the largest logit is there less than its rounding, or about as much."""
+    gen = torch.Generator().manual_seed(3)
+    step = math.ulp(max(abs(at), 2.0 ** -10)) * 2.0 ** 29    # a unit in the last place of fp32
+    x = (at + step * torch.randint(-40, 1, (8, 2500), generator=gen).double()).float().to(dev)
+    for T in (0.01, 0.012, 0.02, 0.03, 0.1, 0.9, 20.0):
+        _check(x, torch.rand(8, generator=gen), T=T * step)
+        _check(x, torch.rand(8, generator=gen), T=T * step, p=0.9, m=0.01)
