@@ -84,7 +84,8 @@ def _sample_cpu(logits, u, temperature, top_k, top_p, min_p):
     vals = vals.double()
     top = vals[:, :1]
     t = (one if temperature is None else temperature).double()[:, None]
-    w = torch.where(vals == top, 1.0, torch.where(top.isposinf(), 0.0, torch.exp((vals - top) / torch.where(t > 0, t, 1.0))))
+    w = torch.exp((vals - top) / torch.where(t > 0, t, 1.0))
+    w = torch.where(vals == top, 1.0, torch.where(top.isposinf() | vals.isneginf(), 0.0, w))      # (also where T is infinite)
     place = torch.arange(V)[None, :]
     if top_k is not None:
         k = top_k.long()[:, None]

@@ -88,3 +88,26 @@ def test_temperatures_next_to_the_logits_own_rounding(dev, at):
     for T in (0.01, 0.012, 0.02, 0.03, 0.1, 0.9, 20.0):
         _check(x, torch.rand(8, generator=gen), T=T * step)
         _check(x, torch.rand(8, generator=gen), T=T * step, p=0.9, m=0.01)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9, 3001])
+def test_an_infinite_temperature_draws_evenly_among_what_is_left(dev, dtype, V):
+    gen = torch.Generator().manual_seed(V)
+    x = (torch.randn(6, V, generator=gen) * 4).to(dtype)
+    x[1, ::2] = float("-inf")
+    x[2, ::3] = float("nan")
+    x[3, 1:] = float("-inf")
+    x[4, 2:7] = torch.finfo(dtype).min
+    x[5, :] = float("-inf")
+    u = torch.rand(6, generator=gen)
+    for k in (0, 3):
+        tokens, lps = sample_rows(x.to(dev), u.to(dev), torch.full((6,), float("inf"), device=dev), torch.full((6,), k, dtype=torch.int32, device=dev))
+        for i in range(5):
+            row = torch.where(x[i].float().isnan(), float("-inf"), x[i].float())
+            order = torch.sort(row, descending=True, stable=True).indices[:int((row > float("-inf")).sum())]
+            order = order[:k] if k else order
+            assert tokens[i].item() == order[int(u[i].item() * len(order))].item()
+            assert abs(lps[i].item() + math.log(len(order))) <= 2.0 ** -24 * math.log(len(order)) + 1e-9
+        assert tokens[5] == 0 and lps[5] == float("-inf")
