@@ -367,6 +367,11 @@ class LLMEngine:
         batches step eagerly, and their pages are not cached."""
         if bank is not None and self.model.ps.tp * self.model.ps.pp * self.model.ps.ep * self.model.ps.cp > 1:
             raise ValueError("adapters of many requests need tensor-, pipeline-, expert- and context-parallel degrees of 1")
+        if bank is not None:
+            views = dict(self.model.named_weights())
+            for t, a in bank.A.items():
+                if t not in views or views[t].shape != (bank.B[t].shape[1], a.shape[2]) or a.device.type != self.device.type or a.dtype != views[t].dtype:
+                    raise ValueError(f"the bank's {t!r} does not fit this engine's model (shape, type or device)")
         self._drain_inflight()
         if any(s.adapter >= 0 for s in [*self.scheduler.waiting, *self.scheduler.running]):
             raise RuntimeError("set_adapters with requests in flight that use the present ones")

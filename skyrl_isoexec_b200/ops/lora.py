@@ -15,6 +15,7 @@ from . import _native
 from . import functional as F
 
 MAX_RANK = 128
+MAX_ADAPTERS = 1024         # in a bank (csrc/lora.cu::kMaxAdapters)
 
 
 class LoraPlan:
@@ -64,6 +65,19 @@ def pad_rank(A: torch.Tensor, B: torch.Tensor, rank: int) -> tuple[torch.Tensor,
     if A.dim() != 2 or B.dim() != 2 or B.shape[1] != r or rank < r:
         raise ValueError(f"pad_rank: A {tuple(A.shape)} and B {tuple(B.shape)} do not fit rank {rank}")
     return torch.nn.functional.pad(A, (0, 0, 0, rank - r)), torch.nn.functional.pad(B, (0, rank - r))
+
+
+def check_bank(adapters: int, rank: int, widths, dtype: torch.dtype) -> None:
+    """Refuse a bank that the kernels cannot compute with. ``widths``: (name, in, out) of every target."""
+    if adapters > MAX_ADAPTERS:
+        raise ValueError(f"lora: at most {MAX_ADAPTERS} adapters in a bank, not {adapters}")
+    if rank % 8 or not 8 <= rank <= MAX_RANK:
+        raise ValueError(f"lora: a bank's rank is a multiple of 8 up to {MAX_RANK}, not {rank}")
+    if dtype != torch.bfloat16:
+        raise ValueError(f"lora: on a GPU the factors are bf16, not {dtype}")
+    for name, inn, out in widths:
+        if inn % 8 or out % 8:
+            raise ValueError(f"lora: {name} is {inn} -> {out}, widths are multiples of 8")
 
 
 def _check(y, x, A, B, scale, plan) -> None:

@@ -143,7 +143,12 @@ class AdapterBank:
         self.scale = torch.tensor(self.scales, dtype=torch.float32, device=dev)
         self.A: dict[str, torch.Tensor] = {}
         self.B: dict[str, torch.Tensor] = {}
-        for t in [n for n in views if any(n in ad.A for ad in adapters.values())]:
+        targets = [n for n in views if any(n in ad.A for ad in adapters.values())]
+        if dev.type == "cuda":               # refused here, not in the middle of an engine's step
+            from ..ops.lora import check_bank
+
+            check_bank(len(adapters), self.rank, [(t, *reversed(views[t].shape)) for t in targets], model.store.flat.dtype)
+        for t in targets:
             out, inn = views[t].shape
             self.A[t] = torch.zeros(len(adapters), self.rank, inn, dtype=views[t].dtype, device=dev)
             self.B[t] = torch.zeros(len(adapters), out, self.rank, dtype=views[t].dtype, device=dev)
