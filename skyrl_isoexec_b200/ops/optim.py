@@ -186,13 +186,23 @@ class TensorAdamW:
             m, v = m * self.state["exp_avg_scale"][per], (v * self.state["exp_avg_sq_scale"][per]).square()
         return m.view(self.params[i].shape), v.view(self.params[i].shape)
 
+    def _shapes(self) -> list:
+        return [tuple(p.shape) for p in self.params]
+
     def state_dict(self) -> dict:
-        return {"step": self.step_count, **{k: v.clone() for k, v in self.state.items()}}
+        return {"step": self.step_count, "shapes": self._shapes(), **{k: v.clone() for k, v in self.state.items()}}
 
     @torch.no_grad()
     def load_state_dict(self, sd: dict) -> None:
+        """Take a ``state_dict()`` of the same tensors in the same order. (``shapes`` says which they were; a state that was
+        put together elsewhere may come without, its buffers laid out by ``offsets``.)"""
         sd = dict(sd)
-        step = int(sd.pop("step"))
+        if "step" not in sd:
+            raise ValueError("TensorAdamW: not a state of this optimizer (no step count)")
+        step, shapes = int(sd.pop("step")), sd.pop("shapes", None)
+        if shapes is not None and [tuple(x) for x in shapes] != self._shapes():
+            at = next((i for i, (a, b) in enumerate(zip(shapes, self._shapes())) if tuple(a) != b), min(len(shapes), len(self.params)))
+            raise ValueError(f"TensorAdamW: the state is of {len(shapes)} tensors, this optimizer has {len(self.params)}, and they differ from number {at} on")
         if set(sd) != set(self.state):
             raise ValueError(f"TensorAdamW: state has {sorted(sd)}, this optimizer {sorted(self.state)}")
         for k, v in sd.items():
