@@ -200,14 +200,14 @@ class TensorAdamW:
         if "step" not in sd:
             raise ValueError("TensorAdamW: not a state of this optimizer (no step count)")
         step, shapes = int(sd.pop("step")), sd.pop("shapes", None)
-        if shapes is not None and [tuple(x) for x in shapes] != self._shapes():
-            at = next((i for i, (a, b) in enumerate(zip(shapes, self._shapes())) if tuple(a) != b), min(len(shapes), len(self.params)))
-            raise ValueError(f"TensorAdamW: the state is of {len(shapes)} tensors, this optimizer has {len(self.params)}, and they differ from number {at} on")
         if set(sd) != set(self.state):
             raise ValueError(f"TensorAdamW: state has {sorted(sd)}, this optimizer {sorted(self.state)}")
         for k, v in sd.items():
             if v.shape != self.state[k].shape or v.dtype != self.state[k].dtype:
                 raise ValueError(f"TensorAdamW: {k} is {tuple(v.shape)} {v.dtype}, expected {tuple(self.state[k].shape)} {self.state[k].dtype}")
+        if shapes is not None and [tuple(x) for x in shapes] != self._shapes():
+            at = next((i for i, (a, b) in enumerate(zip(shapes, self._shapes())) if tuple(a) != b), min(len(shapes), len(self.params)))
+            raise ValueError(f"TensorAdamW: the state is of {len(shapes)} tensors, this optimizer has {len(self.params)}, and they differ from number {at} on")
         for k, v in sd.items():
             self.state[k].copy_(v)
         self.step_count = step

@@ -27,7 +27,7 @@ def test_a_state_of_other_tensors_is_refused(dev, dt, bits):
             b.load_state_dict(sd)
         assert b.step_count == 0 and not any(v.float().any() for v in b.state.values())
     for shapes in (((300,), (10,)), ((300,), (10,), (20, 30), (0,))):
-        with pytest.raises(ValueError, match="differ from number"):
+        with pytest.raises(ValueError, match="differ from number|expected"):
             opt(*shapes).load_state_dict(sd)
     with pytest.raises(ValueError, match="no step count"):
         a.load_state_dict({"state": {}, "param_groups": []})
