@@ -32,7 +32,7 @@ class TensorAdamW:
     Gradients are read from ``grads``, one buffer per parameter that the program fills again for every step (autograd, a
     projection, ``F.gemm_tn(out=...)``); without the argument they are made here, fp32 zeros in one allocation
     (``zero_grad`` clears them). The memory of parameters and gradients is fixed at construction (and kept alive): a step does
-    no per-tensor work on the host, and does not see a ``p.data`` or an entry of ``state`` that was replaced.
+    no per-tensor work on the host, and does not see a ``p.data`` or an entry of ``params``, ``grads`` or ``state`` that was replaced.
 
     ``state_bits=8``: both moments in e4m3 with one scale per 256 elements, the second by its square root, 2 bytes and a bit
     per element instead of 8. ``state`` holds flat buffers in which tensor ``i`` starts at ``offsets[i]`` (a multiple of
@@ -78,7 +78,9 @@ class TensorAdamW:
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("TensorAdamW: two of the parameters share memory")
-        self._memory = [t.detach() for t in (*params, *self.grads)]      # what a step writes and reads stays allocated
+        # what a step writes and reads: stays allocated, and is what it was at construction on either device
+        self._params, self._grads = [p.detach() for p in params], [g.detach() for g in self.grads]
+        self._memory = [*self._params, *self._grads]
         self.step_count = 0
         st = FP8 if state_bits == 8 else torch.float32
         self.state = {"exp_avg": torch.zeros(total, dtype=st, device=dev), "exp_avg_sq": torch.zeros(total, dtype=st, device=dev)}
@@ -87,7 +89,8 @@ class TensorAdamW:
                 self.state[k] = torch.zeros(total // BLOCK, dtype=torch.float32, device=dev)
         if dt == torch.bfloat16:
             self.state["master"] = torch.zeros(total, dtype=torch.float32, device=dev)
-            self.refresh_masters()
+        self._buffers = dict(self.state)
+        self.refresh_masters()
         self._memory += self.state.values()
         if dev.type == "cuda":
             self._tables()
@@ -98,7 +101,7 @@ class TensorAdamW:
     def _tables(self) -> None:
         chunk = _native.lib().ix_tensor_adamw_chunk()
         rows = bytearray()
-        for p, g, off, wd in zip(self.params, self.grads, self.offsets, self.weight_decay):
+        for p, g, off, wd in zip(self._params, self._grads, self.offsets, self.weight_decay):
             vec = int(p.data_ptr() % 16 == 0 and g.data_ptr() % 16 == 0)
             rows += struct.pack("<QQqqfi24x", p.data_ptr(), g.data_ptr(), p.numel(), off, wd, vec)
         n = torch.tensor([-(-p.numel() // chunk) for p in self.params])
@@ -106,7 +109,7 @@ class TensorAdamW:
         piece = torch.arange(len(tensor)) - (n.cumsum(0) - n)[tensor]
         self._table = torch.frombuffer(rows, dtype=torch.uint8).to(self.device)
         self._chunks = torch.stack([tensor, piece], 1).to(torch.int32).to(self.device)
-        st = self.state
+        st = self._buffers
         # everything a step passes that does not change: the buffers are this object's own
         self._args = (self._table.data_ptr(), self._chunks.data_ptr(), len(tensor), int(self.params[0].dtype == torch.float32),
                       int(self.grads[0].dtype == torch.float32), int(self.state_bits == 8), _native.ptr(st.get("master")), st["exp_avg"].data_ptr(),
@@ -115,16 +118,16 @@ class TensorAdamW:
     @torch.no_grad()
     def refresh_masters(self) -> None:
         """Take the masters from the bf16 parameters again (after weights were loaded)."""
-        if "master" in self.state:
-            for p, o in zip(self.params, self.offsets):
-                self.state["master"][o:o + p.numel()].copy_(p.detach().reshape(-1))
+        if "master" in self._buffers:
+            for p, o in zip(self._params, self.offsets):
+                self._buffers["master"][o:o + p.numel()].copy_(p.reshape(-1))
 
     @torch.no_grad()
     def zero_grad(self) -> None:
         if self._own_grad is not None:
             self._own_grad.zero_()
         else:
-            torch._foreach_zero_(self.grads)
+            torch._foreach_zero_(self._grads)
 
     @torch.no_grad()
     def step(self, lr: float | None = None, grad_scale: torch.Tensor | None = None) -> None:
@@ -153,8 +156,8 @@ class TensorAdamW:
 
     def _step_cpu(self, lr, grad_scale) -> None:
         b1, b2 = self.betas
-        st, t = self.state, self.step_count
-        for i, (p, g, o) in enumerate(zip(self.params, self.grads, self.offsets)):
+        st, t = self._buffers, self.step_count
+        for i, (p, g, o) in enumerate(zip(self._params, self._grads, self.offsets)):
             n = p.numel()
             e = o + -(-n // BLOCK) * BLOCK
             x = torch.nn.functional.pad(g.reshape(-1).float(), (0, e - o - n))
@@ -179,18 +182,18 @@ class TensorAdamW:
 
     def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(mean, second moment) of parameter ``i`` in fp32, decoded."""
-        o, n = self.offsets[i], self.params[i].numel()
-        m, v = self.state["exp_avg"][o:o + n].float(), self.state["exp_avg_sq"][o:o + n].float()
+        o, n, st = self.offsets[i], self._params[i].numel(), self._buffers
+        m, v = st["exp_avg"][o:o + n].float(), st["exp_avg_sq"][o:o + n].float()
         if self.state_bits == 8:
             per = torch.arange(o, o + n, device=m.device) // BLOCK
-            m, v = m * self.state["exp_avg_scale"][per], (v * self.state["exp_avg_sq_scale"][per]).square()
-        return m.view(self.params[i].shape), v.view(self.params[i].shape)
+            m, v = m * st["exp_avg_scale"][per], (v * st["exp_avg_sq_scale"][per]).square()
+        return m.view(self._params[i].shape), v.view(self._params[i].shape)
 
     def _shapes(self) -> list:
-        return [tuple(p.shape) for p in self.params]
+        return [tuple(p.shape) for p in self._params]
 
     def state_dict(self) -> dict:
-        return {"step": self.step_count, "shapes": self._shapes(), **{k: v.clone() for k, v in self.state.items()}}
+        return {"step": self.step_count, "shapes": self._shapes(), **{k: v.clone() for k, v in self._buffers.items()}}
 
     @torch.no_grad()
     def load_state_dict(self, sd: dict) -> None:
@@ -200,14 +203,14 @@ class TensorAdamW:
         if "step" not in sd:
             raise ValueError("TensorAdamW: not a state of this optimizer (no step count)")
         step, shapes = int(sd.pop("step")), sd.pop("shapes", None)
-        if set(sd) != set(self.state):
-            raise ValueError(f"TensorAdamW: state has {sorted(sd)}, this optimizer {sorted(self.state)}")
+        if set(sd) != set(self._buffers):
+            raise ValueError(f"TensorAdamW: state has {sorted(sd)}, this optimizer {sorted(self._buffers)}")
         for k, v in sd.items():
-            if v.shape != self.state[k].shape or v.dtype != self.state[k].dtype:
-                raise ValueError(f"TensorAdamW: {k} is {tuple(v.shape)} {v.dtype}, expected {tuple(self.state[k].shape)} {self.state[k].dtype}")
+            if v.shape != self._buffers[k].shape or v.dtype != self._buffers[k].dtype:
+                raise ValueError(f"TensorAdamW: {k} is {tuple(v.shape)} {v.dtype}, expected {tuple(self._buffers[k].shape)} {self._buffers[k].dtype}")
         if shapes is not None and [tuple(x) for x in shapes] != self._shapes():
             at = next((i for i, (a, b) in enumerate(zip(shapes, self._shapes())) if tuple(a) != b), min(len(shapes), len(self.params)))
             raise ValueError(f"TensorAdamW: the state is of {len(shapes)} tensors, this optimizer has {len(self.params)}, and they differ from number {at} on")
         for k, v in sd.items():
-            self.state[k].copy_(v)
+            self._buffers[k].copy_(v)
         self.step_count = step

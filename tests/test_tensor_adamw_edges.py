@@ -36,3 +36,29 @@ def test_a_state_of_other_tensors_is_refused(dev, dt, bits):
     assert b.step_count == 1 and all(torch.equal(a.state[k].float(), b.state[k].float()) for k in a.state)
     sd.pop("shapes")                                         # a state that was put together elsewhere
     b.load_state_dict(sd)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_is_on_the_memory_of_construction_on_every_device(dev, dt, bits):
+    """A parameter's storage, a gradient buffer or an entry of ``state`` that was replaced: the step goes on with the first."""
+    def run(replace):
+        w, g = torch.ones(300, dtype=dt, device=dev), torch.ones(300, device=dev)
+        held, opt = w.detach(), TensorAdamW([w], grads=[g], lr=0.1, state_bits=bits)
+        opt.step()
+        if replace:
+            w.data = torch.zeros(300, dtype=dt, device=dev)
+            opt.grads[0] = torch.full((300,), -7.0, device=dev)
+            for k in opt.state:
+                opt.state[k] = torch.zeros_like(opt.state[k])
+        opt.step()
+        if replace:
+            assert not w.any() and not any(v.float().any() for v in opt.state.values())
+        sd = opt.state_dict()
+        opt.load_state_dict(sd)
+        opt.step()
+        return held, opt.moments(0)
+
+    (a, am), (b, bm) = run(False), run(True)
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(am, bm)) and (a.float() < 0.75).all()
