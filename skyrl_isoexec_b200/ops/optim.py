@@ -55,7 +55,7 @@ class TensorAdamW:
         dev, dt = params[0].device, params[0].dtype          # (a tensor's device always carries its index)
         if dt not in (torch.float32, torch.bfloat16):
             raise ValueError(f"TensorAdamW: parameters are fp32 or bf16, not {dt}")
-        self.device, self.lr, self.betas, self.eps, self.weight_decay, self.state_bits = dev, lr, tuple(betas), eps, decay, state_bits
+        self.device, self.lr, self.betas, self.eps, self._decay, self.state_bits = dev, lr, tuple(betas), eps, tuple(decay), state_bits
         self.params = params
         self.offsets, total = [], 0
         for p in params:
@@ -98,10 +98,15 @@ class TensorAdamW:
     def __reduce_ex__(self, protocol):
         raise TypeError("TensorAdamW is tied to the memory of its parameters: build another one and pass state_dict() on")
 
+    @property
+    def weight_decay(self) -> tuple:
+        """Per parameter. Fixed at construction (it stands in the table on the device); ``lr``, ``betas`` and ``eps`` may be set."""
+        return self._decay
+
     def _tables(self) -> None:
         chunk = _native.lib().ix_tensor_adamw_chunk()
         rows = bytearray()
-        for p, g, off, wd in zip(self._params, self._grads, self.offsets, self.weight_decay):
+        for p, g, off, wd in zip(self._params, self._grads, self.offsets, self._decay):
             vec = int(p.data_ptr() % 16 == 0 and g.data_ptr() % 16 == 0)
             rows += struct.pack("<QQqqfi24x", p.data_ptr(), g.data_ptr(), p.numel(), off, wd, vec)
         n = torch.tensor([-(-p.numel() // chunk) for p in self.params])
@@ -171,7 +176,7 @@ class TensorAdamW:
             v = b2 * v + (1 - b2) * x * x
             master = st["master"][o:o + n] if "master" in st else p.view(-1)
             upd = lr / (1 - b1 ** t) * m[:n] / (v[:n].sqrt() / (1 - b2 ** t) ** 0.5 + self.eps)
-            master.copy_(master * (1 - lr * self.weight_decay[i]) - upd)
+            master.copy_(master * (1 - lr * self._decay[i]) - upd)
             if "master" in st:
                 p.view(-1).copy_(master)
             if self.state_bits == 8:

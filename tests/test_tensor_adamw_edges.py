@@ -62,3 +62,18 @@ def test_a_step_is_on_the_memory_of_construction_on_every_device(dev, dt, bits):
 
     (a, am), (b, bm) = run(False), run(True)
     assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(am, bm)) and (a.float() < 0.75).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_settings_that_a_step_does_not_see_cannot_be_set(dev):
+    opt = TensorAdamW([torch.ones(8, device=dev)], weight_decay=0.1)
+    assert opt.weight_decay == (0.1,)
+    with pytest.raises(AttributeError):
+        opt.weight_decay = [0.0]
+    with pytest.raises(TypeError):
+        opt.weight_decay[0] = 0.0
+    a, b = (TensorAdamW([torch.ones(8, device=dev)], grads=[torch.ones(8, device=dev)], lr=lr, betas=betas) for lr, betas in ((0.5, (0.8, 0.9)), (0.1, (0.9, 0.99))))
+    b.lr, b.betas = 0.5, (0.8, 0.9)
+    a.step()
+    b.step()
+    assert torch.equal(a.params[0], b.params[0])
