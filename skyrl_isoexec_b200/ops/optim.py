@@ -122,10 +122,13 @@ class TensorAdamW:
 
     @torch.no_grad()
     def refresh_masters(self) -> None:
-        """Take the masters from the bf16 parameters again (after weights were loaded)."""
+        """Take the masters from the bf16 parameters again where these are no longer the masters' rounding (after weights were
+        loaded, or one adapter's factors put into a bank): the next step would write the old ones back. Others keep their bits."""
         if "master" in self._buffers:
             for p, o in zip(self._params, self.offsets):
-                self._buffers["master"][o:o + p.numel()].copy_(p.reshape(-1))
+                m, now = self._buffers["master"][o:o + p.numel()], p.reshape(-1)
+                changed = m.to(torch.bfloat16).view(torch.int16) != now.view(torch.int16)
+                m.copy_(torch.where(changed, now.float(), m))
 
     @torch.no_grad()
     def zero_grad(self) -> None:

@@ -129,7 +129,8 @@ class AdapterStore:
 class AdapterBank:
     """The factors of several adapters side by side, per target weight ``A [E, r, in]`` and ``B [E, out, r]`` in the model's type:
     ``r`` is the largest rank, rounded up to a multiple of 8, smaller adapters are filled up with zeros, and an adapter without
-    a target has zeros there. ``trainable``: the factors take gradients (``parameters()``)."""
+    a target has zeros there. ``trainable``: the factors take gradients (``parameters()``), in their own type like any
+    parameter; bf16 ones are summed over micro-batches in bf16."""
 
     def __init__(self, model, adapters: dict[str, LoRAAdapter], trainable: bool = False):
         if not adapters:
@@ -166,7 +167,9 @@ class AdapterBank:
 
     @torch.no_grad()
     def put(self, name: str, ad: LoRAAdapter) -> None:
-        """Take the factors of ``ad`` again (after it stepped on its own) in the place of adapter ``name``."""
+        """Take the factors of ``ad`` again (after it stepped on its own) in the place of adapter ``name``. An optimizer that steps
+        this bank's factors and keeps masters of them (``TensorAdamW`` on bf16) has to take them, too: ``refresh_masters()``;
+        its moments of ``name`` are still those of the factors before."""
         e, r = self.names.index(name), ad.cfg.rank
         if r > self.rank or ad.scale != self.scales[e]:
             raise ValueError(f"AdapterBank: {name!r} changed its rank or scale; build a new bank")
@@ -181,7 +184,8 @@ class AdapterBank:
                 self.B[t][e, :, :r].copy_(ad.B[t])
 
     def adapter(self, name: str) -> LoRAAdapter:
-        """The factors of one adapter, in fp32 and at its own rank."""
+        """The factors of one adapter at its own rank: what the bank holds, in fp32 (rounded to the model's type where that is
+        bf16; an optimizer's fp32 masters stay with the optimizer)."""
         e = self.names.index(name)
         r = self.cfgs[e].rank
         ad = LoRAAdapter(self.cfgs[e])

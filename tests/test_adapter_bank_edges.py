@@ -8,6 +8,7 @@ from skyrl_isoexec_b200.engine.sampler import SamplingParams
 from skyrl_isoexec_b200.models.config import get_config
 from skyrl_isoexec_b200.models.decoder import DecoderLM
 from skyrl_isoexec_b200.ops import lora as ops
+from skyrl_isoexec_b200.ops.optim import TensorAdamW
 from skyrl_isoexec_b200.train.lora import AdapterBank, LoRAAdapter, LoRAConfig
 
 
@@ -56,3 +57,28 @@ def test_an_engine_refuses_a_bank_of_another_model(dev):
             eng.set_adapters(AdapterBank(host, {"x": LoRAAdapter.init(host, LoRAConfig(rank=8))}))
     eng.set_adapters(AdapterBank(model, {"x": LoRAAdapter.init(model, LoRAConfig(rank=8))}))
     eng.set_adapters(None)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_factors_put_into_a_bank_under_an_optimizer(dev):
+    """One tenant's factors are replaced while the bank trains: after refresh_masters() the next step starts from them, and the
+    other tenant's masters keep their bits."""
+    model = _model(dev)
+    a, b = (LoRAAdapter.init(model, LoRAConfig(rank=8, seed=i)) for i in (1, 2))
+    bank = AdapterBank(model, {"a": a, "b": b}, trainable=True)
+    ps = bank.parameters()
+    gen = torch.Generator().manual_seed(0)
+    opt = TensorAdamW(ps, grads=[torch.randn(p.shape, generator=gen).to(dev) for p in ps], lr=1e-4)
+    opt.step()
+    masters = {k: v.clone() for k, v in opt.state.items() if k == "master"}
+    other = {t: bank.A[t][1].detach().clone() for t in bank.A}
+    new = LoRAAdapter.init(model, LoRAConfig(rank=8, seed=9))
+    bank.put("a", new)
+    opt.refresh_masters()
+    opt.step(0.0)                                            # no step: what is written back is what the masters are
+    for t in bank.A:
+        assert torch.equal(bank.A[t][0], new.A[t].to(bank.A[t].dtype)) and torch.equal(bank.A[t][1], other[t])
+    if masters:
+        for p, o in zip(ps, opt.offsets):
+            half = p[1].numel()
+            assert torch.equal(opt.state["master"][o + half:o + 2 * half], masters["master"][o + half:o + 2 * half])

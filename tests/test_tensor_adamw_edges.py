@@ -77,3 +77,25 @@ def test_settings_that_a_step_does_not_see_cannot_be_set(dev):
     a.step()
     b.step()
     assert torch.equal(a.params[0], b.params[0])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_refreshed_masters_take_changed_weights_and_keep_the_others(dev, bits):
+    gen = torch.Generator().manual_seed(0)
+    p = [torch.randn(300, generator=gen).bfloat16().to(dev), torch.randn(7, 9, generator=gen).bfloat16().to(dev), torch.tensor([-0.0, 0.0]).bfloat16().to(dev)]
+    opt = TensorAdamW(p, grads=[torch.randn(t.shape, generator=gen).to(dev) for t in p], lr=1e-3, state_bits=bits)
+    assert opt.state["master"][opt.offsets[2]].item() == 0.0 and torch.signbit(opt.state["master"][opt.offsets[2]])
+    opt.step()
+    before = opt.state["master"].clone()
+    opt.refresh_masters()
+    assert torch.equal(opt.state["master"], before)          # still the parameters' rounding: nothing is lost
+    p[0][10:20] = 3.0
+    p[1][2] = float("nan")
+    opt.refresh_masters()
+    now = opt.state["master"]
+    at = torch.zeros_like(now, dtype=torch.bool)
+    at[10:20], at[opt.offsets[1] + 18:opt.offsets[1] + 27] = True, True
+    assert torch.equal(now[~at], before[~at]) and (now[10:20] == 3.0).all() and now[opt.offsets[1] + 18:opt.offsets[1] + 27].isnan().all()
+    opt.step(0.0)
+    assert (p[0][10:20] == 3.0).all()
