@@ -18,6 +18,7 @@ import torch
 
 from ..models.decoder import DecoderLM, ForwardCtx
 from ..ops import functional as F
+from ..ops import sampling as _sampling
 from ..ops.functional import PAGE
 from .kv_cache import KVCache
 from .sampler import Sampler, SamplingParams
@@ -236,6 +237,8 @@ class LLMEngine:
         n_pages = self.cfg.num_kv_pages or self._auto_pages()
         self.cache = KVCache(self.mcfg, n_pages, self.device, tp=model.ps.tp, layer_ids=model.layer_ids)
         self.scheduler = Scheduler(self.cfg, self.cache)
+        if self.cfg.sample_from_numbers and self.mcfg.vocab_size > _sampling.MAX_VOCAB:
+            raise ValueError(f"sample_from_numbers needs a vocabulary of at most {_sampling.MAX_VOCAB}, not {self.mcfg.vocab_size}")
         self.sampler = Sampler(self.device, self.cfg.seed, self.mcfg.logprob_leaves, from_numbers=self.cfg.sample_from_numbers)
         self.adapters = None            # AdapterBank: requests may name one of its adapters (set_adapters)
         self._next_id = 0

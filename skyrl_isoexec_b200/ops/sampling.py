@@ -13,6 +13,8 @@ import torch
 
 from . import _native
 
+MAX_VOCAB = 1 << 19         # tokens of a row on a GPU (csrc/sample_rows.cu::ix_sample_rows_max_vocab)
+
 
 def _setting(t, name, rows, dtype, device):
     if t is None:
@@ -26,7 +28,7 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor
                 top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(tokens int64 [rows], log-probabilities fp32 [rows]).
 
-    ``logits`` [rows, V] bf16 or fp32; ``u`` fp32 [rows] in ``[0, 1)`` (a number outside is moved to the nearer end, NaN to 0). ``temperature`` fp32 (default
+    ``logits`` [rows, V] bf16 or fp32 (on a GPU V is at most ``MAX_VOCAB``); ``u`` fp32 [rows] in ``[0, 1)`` (a number outside is moved to the nearer end, NaN to 0). ``temperature`` fp32 (default
     1; at or below 0: the largest logit), ``top_k`` int32 (at or below 0: off), ``top_p`` fp32 (1 or more: off), ``min_p`` fp32 (at
     or below 0: off), each [rows] or None. A logit of -inf or NaN is never drawn; a row that has no other gives token 0 with
     log-probability -inf. The log-probability is that of the token in the kept, renormalised distribution, the one it was
@@ -59,8 +61,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor
 def _sample_cuda(logits, u, temperature, top_k, top_p, min_p):
     rows, V = logits.shape
     L = _native.lib()
-    if V > L.ix_sample_rows_max_vocab():
-        raise ValueError(f"sample_rows: a vocabulary of at most {L.ix_sample_rows_max_vocab()}, not {V}")
+    if V > MAX_VOCAB:
+        raise ValueError(f"sample_rows: a vocabulary of at most {MAX_VOCAB}, not {V}")
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     bf16 = logits.dtype == torch.bfloat16

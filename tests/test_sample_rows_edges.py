@@ -111,3 +111,22 @@ def test_an_infinite_temperature_draws_evenly_among_what_is_left(dev, dtype, V):
             assert tokens[i].item() == order[int(u[i].item() * len(order))].item()
             assert abs(lps[i].item() + math.log(len(order))) <= 2.0 ** -24 * math.log(len(order)) + 1e-9
         assert tokens[5] == 0 and lps[5] == float("-inf")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_an_engine_refuses_a_vocabulary_that_the_kernel_does_not_take(dev, monkeypatch):
+    from test_adapters_together import _model
+
+    from skyrl_isoexec_b200.engine.llm_engine import EngineConfig, LLMEngine
+    from skyrl_isoexec_b200.ops import sampling
+
+    if dev == "cuda":
+        from skyrl_isoexec_b200.ops import _native
+
+        assert _native.lib().ix_sample_rows_max_vocab() == sampling.MAX_VOCAB
+    model = _model(dev)
+    LLMEngine(model, EngineConfig(max_num_seqs=2, num_kv_pages=8, sample_from_numbers=True))
+    monkeypatch.setattr(sampling, "MAX_VOCAB", model.cfg.vocab_size - 1)
+    with pytest.raises(ValueError, match="sample_from_numbers needs a vocabulary"):
+        LLMEngine(model, EngineConfig(max_num_seqs=2, num_kv_pages=8, sample_from_numbers=True))
+    LLMEngine(model, EngineConfig(max_num_seqs=2, num_kv_pages=8))
