@@ -1037,7 +1037,8 @@ IX_API int ix_lora_backward(const void* dy, long long ld_dy, const void* x, long
   if (T > 0 && dA != nullptr && g == nullptr) return ixh::fail(ixh::IX_EARG, "lora: the gradient of A needs scratch for g");
   if (T > 0 && dB != nullptr && h == nullptr) return ixh::fail(ixh::IX_EARG, "lora: the gradient of B needs the forward's h");
   if (r < 8 || r > kMaxRank || r % 8) return ixh::fail(ixh::IX_EARG, "lora: rank %d is not a multiple of 8 up to %d", r, kMaxRank);
-  if (K < 8 || N < 8 || K % 8 || N % 8 || ld_dy % 8 || ld_x % 8) return ixh::fail(ixh::IX_EARG, "lora: widths and row strides must be multiples of 8");
+  if (K < 8 || N < 8 || K % 8 || N % 8) return ixh::fail(ixh::IX_EARG, "lora: widths %d and %d must be multiples of 8", K, N);
+  if (T > 0 && (ld_dy % 8 || ld_x % 8)) return ixh::fail(ixh::IX_EARG, "lora: row strides must be multiples of 8");
   if (dx != nullptr || dA != nullptr) {
     const int rc = ix_lora_apply(dy, ld_dy, base, ld_base, dx, ld_dx, B, A, scale, perm, tiles_small, tiles_large, n_tiles, dA != nullptr ? g : nullptr,
                                  T, N, K, r, E, 1, stream);

@@ -4,7 +4,7 @@ import pytest
 import torch
 from test_lora_many_adapters import DEVICES, _make, _reference, _tol
 
-from skyrl_isoexec_b200.ops.lora import LoraPlan, lora_add
+from skyrl_isoexec_b200.ops.lora import LoraPlan, lora_add, lora_linear
 
 
 def _run(y, x, A, B, scale, ids, dout):
@@ -75,3 +75,22 @@ def test_a_bank_larger_than_the_batch_of_adapters(dev, r):
     for name in ("out", "dx"):                           # another order of 32-bit sums, then the same rounding
         assert ((got[name].double() - alone[name].double()).abs() <= 2 * _tol(name, ref[name], mag[name], *shape[:4])).all()
     assert not got["dA"][:63].any() and not got["dB"][:63].any()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("odd", ["x", "dout", "both"])
+def test_an_empty_batch_of_rows_of_a_wider_buffer(dev, odd):
+    """No token, rows with a stride that 8 does not divide: the gradients of the factors are zero."""
+    y, x, A, B, scale, ids, dout = _make(40, 64, 48, 8, 2, "shuffled", dev)
+    wide_x, wide_d = (torch.full((4, w + 9), float("nan"), device=dev).bfloat16() for w in (64, 48))
+    none = slice(2, 2)
+    leaf = (wide_x[none, 3:67] if odd != "dout" else x[:0]).detach().requires_grad_(True)
+    d = wide_d[none, 5:53] if odd != "x" else dout[:0]
+    leaves = [leaf, A.clone().requires_grad_(True), B.clone().requires_grad_(True)]
+    out = lora_add(y[:0], *leaves, scale, LoraPlan(ids[:0], 2))
+    dx, dA, dB = torch.autograd.grad(out, leaves, d)
+    assert out.shape == (0, 48) and dx.shape == (0, 64) and not dA.any() and not dB.any() and dA.shape == A.shape and dB.shape == B.shape
+    w = torch.zeros(48, 64, device=dev).bfloat16()
+    leaves = [leaf.detach().requires_grad_(True), A.clone().requires_grad_(True), B.clone().requires_grad_(True)]
+    out = lora_linear(leaves[0], w, *leaves[1:], scale, LoraPlan(ids[:0], 2))
+    assert out.shape == (0, 48) and not any(g.any() for g in torch.autograd.grad(out, leaves, d))
