@@ -281,6 +281,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, A: torch.Tensor, B: torch.Tens
     _check(None, x, A, B, scale, plan)
     if w.dim() != 2 or w.shape != (B.shape[1], A.shape[2]) or w.dtype != x.dtype or w.device != x.device:
         raise ValueError(f"lora: w {tuple(w.shape)} {w.dtype} does not fit factors of widths {A.shape[2]} and {B.shape[1]}")
+    if x.is_cuda and torch.cuda.current_device() != plan.index:      # (the projection launches on the current device)
+        with torch.cuda.device(plan.index):
+            return lora_linear(x, w, A, B, scale, plan)
     scale = _flat(scale)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or x.requires_grad or w.requires_grad):
         return _LoraLinear.apply(x, w, A, B, scale, plan)

@@ -4,6 +4,7 @@ import pytest
 import torch
 from test_lora_many_adapters import DEVICES, _make, _reference, _tol
 
+from skyrl_isoexec_b200.ops import functional as F
 from skyrl_isoexec_b200.ops.lora import LoraPlan, lora_add, lora_linear
 
 
@@ -94,3 +95,40 @@ def test_an_empty_batch_of_rows_of_a_wider_buffer(dev, odd):
     leaves = [leaf.detach().requires_grad_(True), A.clone().requires_grad_(True), B.clone().requires_grad_(True)]
     out = lora_linear(leaves[0], w, *leaves[1:], scale, LoraPlan(ids[:0], 2))
     assert out.shape == (0, 48) and not any(g.any() for g in torch.autograd.grad(out, leaves, d))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_on_another_device_than_the_current_one(dev, monkeypatch):
+    """The calls run under their tensors' device. (Elsewhere than on two GPUs: the current device only seems to be another.)"""
+    y, x, A, B, scale, ids, dout = _make(40, 64, 48, 8, 2, "shuffled", dev)
+    w = torch.randn(48, 64, generator=torch.Generator().manual_seed(0)).bfloat16().to(dev)
+    plan = LoraPlan(ids, 2)
+    want = [lora_add(y, x, A, B, scale, plan), lora_linear(x, w, A, B, scale, plan)]
+    entered, inside = [], []
+    if dev == "cuda":
+        seen = F.gemm_nt
+
+        class Under:
+            def __init__(self, index):
+                entered.append(index)
+
+            def __enter__(self):
+                inside.append(1)
+
+            def __exit__(self, *_):
+                inside.pop()
+
+        def gemm_nt(*a, **kw):
+            assert inside, "the projection outside its tensors' device"
+            return seen(*a, **kw)
+
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: plan.index if inside else 1 + plan.index)
+        monkeypatch.setattr(torch.cuda, "device", Under)
+        monkeypatch.setattr(F, "gemm_nt", gemm_nt)
+    got = [lora_add(y, x, A, B, scale, plan), lora_linear(x, w, A, B, scale, plan)]
+    leaves = [t.clone().requires_grad_(True) for t in (x, A, B)]
+    out = lora_linear(leaves[0], w, *leaves[1:], scale, plan)
+    monkeypatch.undo()
+    assert torch.equal(out.detach(), want[1]) and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(g.isfinite().all() for g in torch.autograd.grad(out, leaves, dout))
+    assert dev == "cpu" or set(entered) == {plan.index}
