@@ -12,14 +12,16 @@
 // once, y read and out written once, h never goes through memory on the way. The backward's g and dx are the same kernel
 // with the factors read across their rows. h and g are kept in 32 bits until they become operands of the second product:
 // there each is the sum of two bf16 numbers (its rounding and the rest, 16 bits together), so the only rounding to 8 bits
-// that shows is that of the output. Products run on mma.sync (532 TFLOP/s here; rank 16 needs 105 of them at the copy rate,
+// that shows is that of the output (parts that carry all 24 bits move as many results over a rounding border: the 32-bit sums'
+// order does). Products run on mma.sync (532 TFLOP/s here; rank 16 needs 105 of them at the copy rate,
 // rank 64 420): with N or K of 8 to 128 a tcgen05 tile is mostly empty, and rows may lie anywhere. Small tiles take operands
 // straight from global memory in fragments of 16 bytes a lane: a contraction may take its elements in any order as long as
 // both operands agree, so a lane's 8 neighbours feed two products of depth 16.
 //
-// Measured (6.54 TB/s is a copy): 48 tokens of 32 adapters, 4096 -> 6144, rank 16: 7.3 us, of which 5 are the latency of one
-// token's; 8192 tokens, 4096 -> 24576, rank 16: 163 us, 5.3 TB/s; dx the other way 104 us, 4.5 TB/s; dB 79 us, 5.1 TB/s;
-// 4093 tokens, 4096 -> 4096, rank 64: 34 us, 3.2 TB/s, bound by shared memory and the two products of each h.
+// Measured (6.54 TB/s is a copy): 48 tokens of 32 adapters, 4096 -> 6144, rank 16: 7.8 us, of which 5 are the latency of one
+// token's; 8192 tokens, 4096 -> 24576, rank 16: 163 us, 5.3 TB/s; dx the other way 105 us, 4.5 TB/s; dB 81 us, 5.0 TB/s;
+// 4093 tokens, 4096 -> 4096, rank 64: 34 us, 3.2 TB/s, bound by shared memory and the two products of each h; 8192 tokens of 4
+// adapters, 4096 -> 4096, rank 128: 114 us.
 #include "bw_common.cuh"
 #include "host_util.h"
 
@@ -983,7 +985,9 @@ IX_API int ix_lora_apply(const void* in, long long ld_in, const void* base, long
   if (tiles > 65535) return ixh::fail(ixh::IX_ESIZE, "lora: %d tokens of %d adapters make more than 65535 tiles", T, E);
   // CTAs a tile: as many as run together, but not beyond eight steps (small: one a warp) each. 8192 tokens 4096 -> 4096: 44 us
   // with 4 at rank 16 (2: 48, 8: 45), 52 with 2 at rank 32 (4: 66), 61 with 2 at rank 64 (4: 66, 1: 75). Where a tile of rank
-  // up to 16 has a long row to write, once more: 4096 -> 24576 takes 163 us with 8, 190 with 4 (ranks 32 and 64 do not gain)
+  // up to 16 has a long row to write, once more (ranks 32 and 64 do not gain). Rank 16, K 4096, N 4096 / 8192 / 16384 / 24576,
+  // without and with it: 8192 tokens (4 CTAs) 46, 46 / 68, 69 / 127, 114 / 191, 164; 12288 (2 CTAs) 63, 66 / 101, 102 / 183, 187 /
+  // 262, 272; 32768 (1 CTA) 167, 153 / 285, 252 / 550, 455 / 791, 664. Next to the rule's border at 8192 tokens, N 12288: 100, 92
   int c = 1;
   const int widest = (K > N ? K : N) / 32;
   const int together = 148 * (!large || r <= 16 ? 4 : r <= 32 ? 3 : r <= 64 ? 2 : 1);

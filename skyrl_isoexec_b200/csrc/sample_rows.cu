@@ -18,11 +18,11 @@
 // steps below the maximum with counts and weights, then the step in question digit by digit.
 //
 // A row is read for the histogram and for the token's place, the second time from L2 or shared memory. Measured: one bf16 row of
-// 151936 17 us, 67 rows of 128256 27 us, which is the latency of their steps; 512 rows of 151936 104 us: a turn of 296 rows
+// 151936 19 us, 67 rows of 128256 27 us, of which 17 are the latency of their steps; 512 rows of 151936 106 us: a turn of 296 rows
 // takes 50 us, 27 of them reading and counting (a warp's 32 atomics 1.5 ns, 14 us in all, beside 14 of reading), 9 looking for
-// the token, and the rest the look ahead, sums in 64 bits and waiting
-// on each other. 24 fp32 rows of 248320 with 3 % of the tokens left 48 us, 256 full ones of 151936
-// 303 us: there every token's weight is computed in 64 bits (6 ns for a warp's).
+// the token, and the rest the look ahead, sums in 64 bits and waiting on each other. 24 fp32 rows of 248320 with 3 % of the
+// tokens left 49 us, 256 full ones of 151936 299 us: there every token's weight is computed in 64 bits (6 ns for a warp's), by a
+// kernel that spills (two CTAs a multiprocessor hold it to 64 registers).
 #include "bw_common.cuh"
 #include "host_util.h"
 
@@ -205,7 +205,7 @@ struct Row {                          // what a row asks for
 
 __device__ __forceinline__ double weight(float x, float top, double T) { return x == top ? 1.0 : exp((static_cast<double>(x) - static_cast<double>(top)) / T); }
 
-// 2^-t for t >= 0: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven implementation of the
+// 2^-t for t > -1/64: 2^-(n / 64) from a table, the rest by its series, six terms (Tang, "Table-driven implementation of the
 // exponential function in IEEE floating-point arithmetic", 1989); a third of exp's work in 64 bits, good to 2e-14 (t itself is
 // rounded to 2^-47)
 __device__ __forceinline__ void fill_table(double* table) {
