@@ -89,8 +89,9 @@ class TensorAdamW:
                 self.state[k] = torch.zeros(total // BLOCK, dtype=torch.float32, device=dev)
         if dt == torch.bfloat16:
             self.state["master"] = torch.zeros(total, dtype=torch.float32, device=dev)
+            for p, o in zip(self._params, self.offsets):
+                self.state["master"][o:o + p.numel()].copy_(p.reshape(-1))
         self._buffers = dict(self.state)
-        self.refresh_masters()
         self._memory += self.state.values()
         if dev.type == "cuda":
             self._tables()

@@ -31,7 +31,7 @@ def _rows(V, gen):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("V", [9001, pytest.param(60001, marks=pytest.mark.gpu), pytest.param(151936, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("V", [9001, *(pytest.param(v, marks=pytest.mark.gpu) for v in (60001, 151936, 524288))])
 def test_a_row_has_the_same_bits_in_every_batch(dev, dtype, V):
     if dev == "cpu" and V > 10000:
         pytest.skip("no other path there")
